@@ -17,7 +17,10 @@ OBJDIR = os.path.join(HERE, "lib", "obj")
 LIB = os.path.join(LIBDIR, "liblt_amd.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result"]
+# -packed-fp32-ops: hipcc forms v_pk_add / mul / fma_f32 from ordinary float code by itself, and some operand forms of those have given wrong
+# results on gfx950 now and then without an error: no kernel of this library contains them
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
@@ -34,7 +37,7 @@ def sources() -> list[str]:
 def _newest_header() -> float:
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     hs += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
-    return max(os.path.getmtime(h) for h in hs)
+    return max(os.path.getmtime(h) for h in hs + [os.path.abspath(__file__)])   # (the compiler flags stand in this file)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -267,7 +267,7 @@ __device__ __forceinline__ void fwd_tile(const char* ldsK, const char* ldsV, int
 // moves only when a tile's row maximum exceeds it by more than 8 octaves (first tile: from -inf), so that on the later tiles the 32
 // accumulator multiplies, the alpha exponential and the lsum rescale are skipped by a wave-uniform branch (probabilities stay <= 2^8:
 // exact in fp32, the same relative precision in bf16; O / lsum and lse = m * scale + ln(lsum) do not depend on which reference was
-// used).  (3) The scale-subtract and the row sum run on fp32 pairs (v_pk_fma_f32 / v_pk_add_f32).  ~110 VALU issue slots per tile against
+// used).  (3) Two row sums, so that the additions do not wait for one another.  ~125 VALU issue slots per tile against
 // ~190 for fwd_tile: N = 197 forward 97 -> 79 us (profiles/r04_attn_fwd_b2.log).
 __device__ __forceinline__ void fwd_tile2(const char* ldsK, const char* ldsV, int tt, int key0, int N, float c, const bf16x8 (&qf)[4],
                                           float& m, float& lsum, f32x16 (&o)[2], int hi) {
@@ -293,18 +293,16 @@ __device__ __forceinline__ void fwd_tile2(const char* ldsK, const char* ldsV, in
 #pragma unroll
     for (int e = 0; e < 16; ++e) { o[0][e] *= alpha; o[1][e] *= alpha; }
   }
-  const f32x2 cc = {c, c}, nmc = {-m * c, -m * c};
-  f32x2 rs2 = {0.f, 0.f};
+  const float nmc = -m * c;
+  float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; e += 2) {
-    f32x2 v = {s[e], s[e + 1]};
-    v = v * cc + nmc;
-    v[0] = __builtin_amdgcn_exp2f(v[0]);
-    v[1] = __builtin_amdgcn_exp2f(v[1]);
-    rs2 += v;
-    s[e] = v[0]; s[e + 1] = v[1];
+    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, nmc));
+    s[e + 1] = __builtin_amdgcn_exp2f(fmaf(s[e + 1], c, nmc));
+    rs0 += s[e];
+    rs1 += s[e + 1];
   }
-  float rs = rs2[0] + rs2[1];
+  float rs = rs0 + rs1;
   rs += __shfl_xor(rs, 32, 64);
   lsum += rs;
   const bf16x8 p0 = pack8(s, 0), p1 = pack8(s, 8);

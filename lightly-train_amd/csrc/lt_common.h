@@ -109,11 +109,10 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
   return fmaf(x * 0.3989422804014327f, e, cdf);
 }
 
-// The same evaluation on a PAIR of values, written on 2-vectors so that the rational / polynomial part compiles to
-// v_pk_fma_f32 / v_pk_mul_f32 (two fp32 operations per lane and issue slot); constants folded (1/sqrt2 into p, 1/2 into the
-// polynomial, -log2(e)/2 into the exponent: v_exp_f32 is a base-2 exponential).  The GELU epilogues of the token GEMMs are
-// VALU-bound, not HBM-bound -- storing the pre-activations as a second output costs nothing, the GELU arithmetic costs 72 us
-// of a 391-us fc1 launch (tools/gelu_probe.py) -- so issue slots are what this buys: 33 per pair instead of 2 x 22.
+// The same evaluation on a PAIR of values; constants folded (1/sqrt2 into p, 1/2 into the polynomial, -log2(e)/2 into the exponent:
+// v_exp_f32 is a base-2 exponential).  The GELU epilogues of the token GEMMs are VALU-bound, not HBM-bound -- storing the pre-activations as
+// a second output costs nothing, the GELU arithmetic cost 72 us of a 391-us fc1 launch (tools/gelu_probe.py) -- so issue slots are what the
+// folding buys.  (The library is built without packed fp32 instructions: a pair is two scalar chains.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_parts2(f32x2 x, f32x2& h, f32x2& ex) {   // h = erfc(|x| / sqrt2) / 2,  ex = exp(-x^2 / 2)
   const f32x2 one = {1.f, 1.f};
@@ -132,7 +131,7 @@ __device__ __forceinline__ void gelu_parts2(f32x2 x, f32x2& h, f32x2& ex) {   //
 // each on |x| <= X0 = 4.5 (least-squares fit on Chebyshev nodes, tools/gelu_fit.py), x clamped beyond.  fp32 Horner against float64:
 // |Phi| error 2.4e-7 (A&S 7.1.26: 1.5e-7), |GELU| 1.1e-6, |GELU'| 2.9e-6 inside; outside, Phi stays at Phi(+-4.5) = 1 - 3.4e-6 | 3.4e-6
 // and GELU' at 1 + 6.9e-5 | -6.9e-5 -- all far below the bf16 rounding (2^-9 relative) of the values these multiply.
-// 17 issue slots per pair, no transcendental, against 33 + 4 quarter-rate ones.
+// No transcendental, against 4 quarter-rate ones.
 #define LT_GELU_X0 4.5f
 template <bool GRAD>
 __device__ __forceinline__ f32x2 gelu_half_plus_odd2(float a, float b) {     // Phi(x) | GELU'(x) on the clamped pair
