@@ -208,6 +208,38 @@ int lt_attention_bwd(const void* qkv, const void* out_bf16, const void* dout_bf1
                      void* dqkv, int B, int N, int H, int dh, float scale, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Cross attention: queries q [B, Nq, H, dh] against the keys / values k, v [B, Nk, Hkv, dh] of another sequence (an encoder's states), beside
+ * the packed self-attention above.  S = scale * q k^T, P = softmax(S) over the visible keys, out = P v, lse = ln sum exp S (f32 [B, H, Nq],
+ * contiguous).  H % Hkv == 0: query head h reads key head h / (H / Hkv).
+ *   dtype      LT_DT_BF16 | LT_DT_F16 of q, k, v, out, dout, dq, dk, dv; scores, statistics and sums are fp32
+ *   dh         8 .. 128, a multiple of 8, last dimension contiguous; s?? = element strides of (batch, token, head), multiples of 8, pointers
+ *              16-byte aligned: views into a packed projection are read and written in place.  Stride 0 (a broadcast input) is allowed for
+ *              inputs; outputs must not overlap each other or an input
+ *   key_lens   int32 [B] or NULL: keys >= key_lens[b] (clamped to 0 .. Nk) are not visible;  key_mask uint8 [B, Nk] or NULL: 0 = not visible.
+ *              Keys that are not visible are not multiplied (their k, v may hold anything) and receive zero gradients; a row without any
+ *              visible key gives out = 0, lse = -inf, dq = 0 and adds nothing to dk, dv
+ *   ws         16-byte aligned scratch of at least lt_cross_attention_*_ws_floats(...) floats (may be 0: NULL), not read before it is written;
+ *              calls that may run at the same time (other streams, other captured graphs) need their own
+ * The backward needs out and lse as the forward left them.  Sums over workgroups are added in a fixed order: results are bitwise reproducible.
+ * ------------------------------------------------------------------------------------------ */
+enum { LT_DT_BF16 = 0, LT_DT_F16 = 1, LT_DT_F32 = 2 };
+typedef struct lt_cross_attention_desc {
+  const void* q; const void* k; const void* v;
+  void* out;                      /* written by the forward, read by the backward */
+  float* lse;                     /* forward: may be NULL */
+  const int32_t* key_lens; const uint8_t* key_mask;
+  const void* dout; void* dq; void* dk; void* dv;   /* backward only */
+  int64_t sq[3], sk[3], sv[3], so[3], sdo[3], sdq[3], sdk[3], sdv[3];
+  int B, Nq, Nk, H, Hkv, dh, dtype;
+  float scale;                    /* > 0 */
+  float* ws; int64_t ws_floats;
+} lt_cross_attention_desc;
+int64_t lt_cross_attention_fwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh);
+int64_t lt_cross_attention_bwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh);
+int lt_cross_attention_fwd(const lt_cross_attention_desc* d, void* stream);
+int lt_cross_attention_bwd(const lt_cross_attention_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Projection head pieces (dinov2_head.py:54-58,66-71)
  * ------------------------------------------------------------------------------------------ */
 /* y = x / max(||x||, eps) per row; outputs bf16 y and the f32 inverse norm */

@@ -25,10 +25,20 @@ class GemmDesc(C.Structure):
     ]
 
 
+class CrossAttentionDesc(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("out", vp), ("lse", vp), ("key_lens", vp), ("key_mask", vp),
+        ("dout", vp), ("dq", vp), ("dk", vp), ("dv", vp),
+        ("sq", i64 * 3), ("sk", i64 * 3), ("sv", i64 * 3), ("so", i64 * 3), ("sdo", i64 * 3), ("sdq", i64 * 3), ("sdk", i64 * 3), ("sdv", i64 * 3),
+        ("B", i32), ("Nq", i32), ("Nk", i32), ("H", i32), ("Hkv", i32), ("dh", i32), ("dtype", i32), ("scale", f32),
+        ("ws", vp), ("ws_floats", i64),
+    ]
+
+
 EPI_BF16, EPI_BF16_GELU, EPI_RESID, EPI_F32, EPI_BF16_GELUGRAD, EPI_F32_ACCUM = range(6)
 ABI_VERSION = 5   # lt_abi_version() of include/lt_amd.h this binding was written against
 
-# name -> argtypes (every function returns int status except lt_last_error)
+# name -> argtypes (every function returns an int status, except lt_last_error and the sizes *_ws_floats)
 SIGNATURES: dict[str, list[Any]] = {
     "lt_abi_version": [],
     "lt_device_info": [C.c_char_p, i32, C.POINTER(i32), C.POINTER(i32)],
@@ -66,6 +76,10 @@ SIGNATURES: dict[str, list[Any]] = {
     "lt_fill_f32": [vp, f32, i64, vp],
     "lt_scale_f32": [vp, f32, i64, vp],
     "lt_attention_fwd": [vp, vp, vp, i32, i32, i32, i32, f32, vp],
+    "lt_cross_attention_fwd_ws_floats": [i32, i32, i32, i32, i32, i32],
+    "lt_cross_attention_bwd_ws_floats": [i32, i32, i32, i32, i32, i32],
+    "lt_cross_attention_fwd": [C.POINTER(CrossAttentionDesc), vp],
+    "lt_cross_attention_bwd": [C.POINTER(CrossAttentionDesc), vp],
     "lt_attention_bwd": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp],
     "lt_l2norm_fwd": [vp, vp, vp, i32, i32, f32, vp],
     "lt_l2norm_bwd": [vp, vp, vp, vp, i32, i32, vp],
@@ -155,7 +169,7 @@ def load() -> C.CDLL:
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError = ABI mismatch, also loud
         fn.argtypes = argtypes
-        fn.restype = C.c_int
+        fn.restype = i64 if name.endswith("_ws_floats") else C.c_int
     if lib.lt_abi_version() != ABI_VERSION:   # a stale build of another signature set would corrupt arguments silently
         raise LtAmdError(f"{LIB_PATH} has ABI version {lib.lt_abi_version()}, this package binds version {ABI_VERSION}: rebuild it")
     _lib = lib

@@ -1,0 +1,1022 @@
+// Cross attention for gfx950: queries q [B, Nq, H, dh] against the keys / values k, v [B, Nk, Hkv, dh] of another sequence (an encoder's states),
+// forward and backward, bf16 or f16 operands, fp32 scores, statistics and accumulators; the score matrix never reaches memory.
+//   S = scale * q k^T (keys that are not visible: -inf), P = softmax(S), O = P V, lse = ln sum exp S;  a row that sees no key: O = 0, lse = -inf
+//   D = rowsum(dO * O), dV = P^T dO, dS = P * (dO V^T - D), dQ = scale * dS K, dK = scale * dS^T Q
+// H / Hkv = G query heads share a key head: the G * Nq query rows of a (batch entry, key head) are one matrix, row r = (head r / Nq, query r % Nq),
+// so the shared heads read their K / V once and their gradients are summed in registers.
+//
+// All products are v_mfma_f32_32x32x16 (A: lane l holds row l % 32, k-slots 8 (l / 32) .. + 7; C: lane -> column l % 32, register e -> row
+// crow(e)).  A C tile whose contraction index lies in the registers is, packed to 16 bits, the next product's B operand without any data movement
+// (the k-slot order {4h .. 4h + 3, 8 + 4h .. 8 + 4h + 3} it implies is applied to the other operand too), so the tiles are formed as
+//   forward   S^T = K Q^T  (lane -> query)  ->  O^T  = V^T P^T      softmax statistics are per lane + one exchange between the wave's halves
+//   dQ        S^T, dP^T = V dO^T            ->  dQ^T = K^T dS^T
+//   dK / dV   S = Q K^T, dP = dO V^T (lane -> key)  ->  dV^T = dO^T P, dK^T = Q^T dS
+// Operands whose contraction index is the token index are read from LDS through ds_read_b64_tr_b16 ("T image": [4 tokens][16 d] pieces of 128 B),
+// the others from padded rows (stride 2 * 32 HD + 16 B: 16 consecutive rows land on 16 different 16-byte bank groups).
+// Keys that are not visible are staged as zeros (what the caller's padding holds is never multiplied) and their scores start at -inf.
+#include "lt_common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float M_NONE = -1e30f;   // running maximum before the first visible key (finite: -inf - -inf never forms)
+constexpr int NT = 256;            // threads per workgroup, four waves
+constexpr int KC = 64;             // tokens per LDS chunk of the tiled kernels
+constexpr float P_UP = 4096.f;     // f16 probabilities of the backward are kept times 2^12: 1 / Nk of a long cache would be subnormal
+
+struct Strides { int64_t b, n, h; };
+struct XArgs {
+  const uint16_t *q, *k, *v, *o, *dout;
+  uint16_t *out, *dq, *dk, *dv;
+  float *lse, *ws, *delta;
+  const int32_t* klen;
+  const uint8_t* kmask;
+  Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  int B, Nq, Nk, H, Hkv, G, R, dh;
+  float scale;
+  int splits, tiles;   // work items along the contracted axis | row (key) tiles per (batch entry, key head)
+};
+
+template <bool F16> __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {   // both round to nearest even
+  if constexpr (F16) { f16x2 v; v[0] = (_Float16)a; v[1] = (_Float16)b; return __builtin_bit_cast(uint32_t, v); }
+  else return pack_bf2(a, b);
+}
+template <bool F16> __device__ __forceinline__ float to_f(short x) {
+  if constexpr (F16) return (float)__builtin_bit_cast(_Float16, x);
+  else return bf2f((uint16_t)x);
+}
+template <bool F16> __device__ __forceinline__ s16x8 pack8(const f32x16& p, int off) {
+  const uint4 u = make_uint4(pack2<F16>(p[off], p[off + 1]), pack2<F16>(p[off + 2], p[off + 3]), pack2<F16>(p[off + 4], p[off + 5]),
+                             pack2<F16>(p[off + 6], p[off + 7]));
+  return __builtin_bit_cast(s16x8, u);
+}
+__device__ __forceinline__ f32x16 splat(float x) {
+  f32x16 r;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r[e] = x;
+  return r;
+}
+__device__ __forceinline__ int lane() { return threadIdx.x & 63; }
+__device__ __forceinline__ int crow(int e, int hi) { return (e & 3) + 8 * (e >> 2) + 4 * hi; }
+__device__ __forceinline__ float half_max(float x) {   // over the two lanes l, l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ s16x8 ld8(const uint16_t* p, bool ok) {
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if (ok) u = *reinterpret_cast<const uint4*>(p);
+  return __builtin_bit_cast(s16x8, u);
+}
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); __builtin_amdgcn_wave_barrier(); }   // lgkmcnt(0)
+
+// ---- LDS images ------------------------------------------------------------------------------------------------------------------
+template <int HD> constexpr int row_stride() { return HD * 64 + 16; }
+template <int HD> __device__ __forceinline__ s16x8 row_frag(const char* img, int tile, int ks) {
+  const int l = lane();
+  return *reinterpret_cast<const s16x8*>(img + (tile * 32 + (l & 31)) * row_stride<HD>() + (2 * ks + (l >> 5)) * 16);
+}
+template <int HD> __device__ __forceinline__ int tr_off(int r, int c) {   // 16-byte chunk c of token r in the T image
+  return ((r >> 2) * (2 * HD) + (c >> 1)) * 128 + ((((r & 3) + (c >> 1)) & 3) << 5) + ((c & 1) << 4);
+}
+// rows = 32 d (block db), k-slots = 16 tokens from tok16 (a multiple of 16) in the C-layout slot order
+template <int HD> __device__ __forceinline__ s16x8 tr_frag(const char* img, int db, int tok16) {
+  const int l = lane(), i = l & 15, b = db * 2 + ((l >> 4) & 1), hi = l >> 5;
+  const int inner = ((((i >> 2) + b) & 3) << 5) + ((i & 3) << 3), q = (tok16 >> 2) + hi;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(img + (q * 2 * HD + b) * 128 + inner));
+  const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(img + ((q + 2) * 2 * HD + b) * 128 + inner));
+  return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// KC tokens between memory and the images, through registers (the next chunk's loads stay in flight while a chunk is computed)
+template <int HD> struct Chunk {
+  static constexpr int CPR = 4 * HD, PER = KC * CPR / NT;
+  uint4 u[PER];
+  __device__ __forceinline__ void load_keys(const uint16_t* base, int64_t sn, int tok0, int end, const uint8_t* mask, int dh) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR, tok = tok0 + r;
+      u[i] = make_uint4(0, 0, 0, 0);
+      if (tok < end && c * 8 < dh && (!mask || mask[tok])) u[i] = *reinterpret_cast<const uint4*>(base + tok * sn + c * 8);
+    }
+  }
+  __device__ __forceinline__ void load_rows(const uint16_t* base, const Strides& s, int r0, int R, int Nq, int dh) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int idx = threadIdx.x + NT * i, r = r0 + idx / CPR, c = idx % CPR;
+      u[i] = make_uint4(0, 0, 0, 0);
+      if (r < R && c * 8 < dh) {
+        const int g = r / Nq, n = r - g * Nq;
+        u[i] = *reinterpret_cast<const uint4*>(base + n * s.n + g * s.h + c * 8);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_rows(char* img) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR;
+      *reinterpret_cast<uint4*>(img + r * row_stride<HD>() + c * 16) = u[i];
+    }
+  }
+  __device__ __forceinline__ void store_tr(char* img) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR;
+      *reinterpret_cast<uint4*>(img + tr_off<HD>(r, c)) = u[i];
+    }
+  }
+};
+template <int HD> constexpr int row_img() { return KC * row_stride<HD>(); }
+template <int HD> constexpr int tr_img() { return KC * HD * 64; }
+
+// the workgroups of one (batch entry, key head) land on one XCD (workgroup i runs on XCD i % 8): they share its K / V in that L2
+__device__ __forceinline__ bool my_item(const XArgs& a, int per, int& bh, int& item) {
+  const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  bh = (i / per) * 8 + x;
+  item = i % per;
+  return bh < a.B * a.Hkv;
+}
+__device__ __forceinline__ int key_end(const XArgs& a, int b) { return a.klen ? min(max(a.klen[b], 0), a.Nk) : a.Nk; }
+
+// accumulators acc[HD] in C layout (lane -> row, registers -> d) to 16-bit rows / fp32 partial rows
+template <bool F16, int HD> __device__ __forceinline__ void put_row(uint16_t* dst, const f32x16 (&acc)[HD], float mul, int dh) {
+  const int hi = lane() >> 5;
+#pragma unroll
+  for (int db = 0; db < HD; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hi;
+      if (d < dh) *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack2<F16>(acc[db][4 * g] * mul, acc[db][4 * g + 1] * mul),
+                                                                  pack2<F16>(acc[db][4 * g + 2] * mul, acc[db][4 * g + 3] * mul));
+    }
+}
+template <int HD> __device__ __forceinline__ void put_partial(float* dst, const f32x16 (&acc)[HD], float mul, int dh) {
+  const int hi = lane() >> 5;
+#pragma unroll
+  for (int db = 0; db < HD; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = db * 32 + 8 * g + 4 * hi;
+      if (d < dh) *reinterpret_cast<float4*>(dst + d) = make_float4(acc[db][4 * g] * mul, acc[db][4 * g + 1] * mul, acc[db][4 * g + 2] * mul, acc[db][4 * g + 3] * mul);
+    }
+}
+
+// ================================================================================================================== forward
+// One online-softmax step of one 32-query tile over NK 32-key tiles of raw scores s (base 2, reference m in raw-score units that moves only when a
+// row's maximum passes it by more than 8 octaves: probabilities stay <= 2^8, exact in fp32 and bf16 / f16 safe).  lsum is per lane (the two halves
+// of a row are added once, at the end).
+template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[NK], float c, float& m, float& lsum, f32x16 (&o)[HD]) {
+  float mx = s[0][0];
+#pragma unroll
+  for (int t = 0; t < NK; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+  mx = half_max(mx);
+  const bool grow = (mx - m) * c > 8.f;
+  if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+    const float mn = grow ? mx : m, alpha = __builtin_amdgcn_exp2f((m - mn) * c);
+    lsum *= alpha;
+    m = mn;
+#pragma unroll
+    for (int db = 0; db < HD; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+  }
+  const float nmc = -m * c;
+  float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+  for (int t = 0; t < NK; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, nmc));
+      s[t][e + 1] = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], c, nmc));
+      r0 += s[t][e];
+      r1 += s[t][e + 1];
+    }
+  lsum += r0 + r1;
+}
+
+// Tiled forward: a workgroup owns 4 waves x QT x 32 query rows of one (batch entry, key head) and walks its share of the keys in chunks of 64.
+template <bool F16, int HD, int QT>
+__global__ __launch_bounds__(NT) void xattn_fwd_kernel(const XArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[2 * (row_img<HD>() + tr_img<HD>() + KC * 4)];
+  constexpr int BUF = row_img<HD>() + tr_img<HD>() + KC * 4;
+  int bh, item;
+  if (!my_item(a, a.tiles * a.splits, bh, item)) return;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, split = item / a.tiles;
+  const int wave = threadIdx.x >> 6, l = lane(), hi = l >> 5;
+  const int kend = key_end(a, b), chunks = (kend + KC - 1) / KC, per = (chunks + a.splits - 1) / a.splits;
+  const int c_lo = min(split * per, chunks), c_hi = min(c_lo + per, chunks);
+  const uint16_t* kb = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
+  const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
+
+  Chunk<HD> kr, vr;
+  float bias = 0.f;
+  auto load = [&](int c) {
+    kr.load_keys(kb, a.sk.n, c * KC, kend, mask, a.dh);
+    vr.load_keys(vb, a.sv.n, c * KC, kend, mask, a.dh);
+    if (threadIdx.x < KC) { const int key = c * KC + threadIdx.x; bias = key < kend && (!mask || mask[key]) ? 0.f : -INFINITY; }
+  };
+  auto store = [&](int buf) {
+    kr.store_rows(smem + buf * BUF);
+    vr.store_tr(smem + buf * BUF + row_img<HD>());
+    if (threadIdx.x < KC) *reinterpret_cast<float*>(smem + buf * BUF + row_img<HD>() + tr_img<HD>() + threadIdx.x * 4) = bias;
+  };
+  if (c_lo < c_hi) load(c_lo);
+  s16x8 qf[QT][2 * HD];
+  f32x16 o[QT][HD];
+  float m[QT], lsum[QT];
+  const int row0 = (tile * 4 + wave) * 32 * QT;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + t * 32 + (l & 31), g = r / a.Nq, n = r - g * a.Nq;
+    const uint16_t* p = a.q + b * a.sq.b + n * a.sq.n + (int64_t)(hk * a.G + g) * a.sq.h;
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) qf[t][ks] = ld8(p + ks * 16 + hi * 8, r < a.R && ks * 16 + hi * 8 < a.dh);
+#pragma unroll
+    for (int db = 0; db < HD; ++db) o[t][db] = splat(0.f);
+    m[t] = M_NONE;
+    lsum[t] = 0.f;
+  }
+  const float c = a.scale * LOG2E;
+  if (c_lo < c_hi) store(0);
+  __syncthreads();
+  for (int ch = c_lo; ch < c_hi; ++ch) {
+    const int buf = (ch - c_lo) & 1;
+    const bool more = ch + 1 < c_hi;
+    if (more) load(ch + 1);
+    const char* K = smem + buf * BUF;
+    const char* V = K + row_img<HD>();
+    const float* bs = reinterpret_cast<const float*>(V + tr_img<HD>());
+    if (row0 < a.R) {
+      const bool biased = mask || (ch + 1) * KC > kend;
+      f32x16 s[QT][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16 init = splat(0.f);
+        if (biased) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 x = *reinterpret_cast<const float4*>(bs + t * 32 + 8 * g + 4 * hi);
+            init[4 * g] = x.x; init[4 * g + 1] = x.y; init[4 * g + 2] = x.z; init[4 * g + 3] = x.w;
+          }
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[qt][t] = init;
+#pragma unroll
+        for (int ks = 0; ks < 2 * HD; ++ks) {
+          const s16x8 kf = row_frag<HD>(K, t, ks);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt][t] = mma<F16>(kf, qf[qt][ks], s[qt][t]);
+        }
+      }
+      s16x8 p[QT][4];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        soft_step<HD, 2>(s[qt], c, m[qt], lsum[qt], o[qt]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) { p[qt][2 * t] = pack8<F16>(s[qt][t], 0); p[qt][2 * t + 1] = pack8<F16>(s[qt][t], 8); }
+      }
+#pragma unroll
+      for (int db = 0; db < HD; ++db)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const s16x8 vf = tr_frag<HD>(V, db, k * 16);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) o[qt][db] = mma<F16>(vf, p[qt][k], o[qt][db]);
+        }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + t * 32 + (l & 31), g = r / a.Nq, n = r - g * a.Nq;
+    const float ls = half_sum(lsum[t]);
+    if (r >= a.R) continue;
+    if (a.splits > 1) {
+      const int64_t rows = (int64_t)a.B * a.Hkv * a.R, row = split * rows + (int64_t)bh * a.R + r;
+      put_partial<HD>(a.ws + row * a.dh, o[t], 1.f, a.dh);
+      if (hi == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * a.dh + row * 2) = make_float2(m[t], ls);
+    } else {
+      const int h = hk * a.G + g;
+      put_row<F16, HD>(a.out + b * a.so.b + n * a.so.n + h * a.so.h, o[t], ls != 0.f ? 1.f / ls : 0.f, a.dh);
+      if (hi == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + n] = ls != 0.f ? m[t] * a.scale + __logf(ls) : -INFINITY;
+    }
+  }
+}
+
+// Few rows (R <= 32: pooling by one query, one new token): the waves share the one row tile and split the KEYS.  K fragments are rows and come
+// straight from memory, V passes through a wave-private T image; the next tile's loads are in flight while a tile is computed.  Bound by reading
+// K / V: the padded matrix work of a 32-key tile (8 HD MFMAs) hides under its 8 KiB * HD / 2 of loads.
+template <int HD> struct KeyTile {
+  s16x8 f[2 * HD];
+  __device__ __forceinline__ void load(const uint16_t* base, int64_t sn, int key, bool ok, int dh) {
+    const int hi = lane() >> 5;
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) f[ks] = ld8(base + key * sn + ks * 16 + hi * 8, ok && ks * 16 + hi * 8 < dh);
+  }
+  __device__ __forceinline__ void store_tr(char* img) const {   // token l % 32, chunk 2 ks + hi
+    const int l = lane();
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) *reinterpret_cast<s16x8*>(img + tr_off<HD>(l & 31, 2 * ks + (l >> 5))) = f[ks];
+  }
+};
+
+template <bool F16, int HD>
+__global__ __launch_bounds__(NT) void xattn_fwd_few_kernel(const XArgs a) {
+  constexpr int OST = HD * 32 + 4;   // floats between the rows of a wave's partial output
+  __shared__ __attribute__((aligned(16))) char smem[4 * 32 * OST * 4 + 4 * 32 * 8];
+  int bh, split;
+  if (!my_item(a, a.splits, bh, split)) return;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int wave = threadIdx.x >> 6, l = lane(), hi = l >> 5;
+  const int kend = key_end(a, b), tiles = (kend + 31) / 32, per = (tiles + a.splits - 1) / a.splits;
+  const int t_lo = min(split * per, tiles), t_hi = min(t_lo + per, tiles);
+  const uint16_t* kb = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
+  const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
+  char* img = smem + wave * (32 * HD * 64);
+
+  KeyTile<HD> kf, vf;
+  bool ok = false;
+  auto load = [&](int t) {
+    const int key = t * 32 + (l & 31);
+    ok = t < t_hi && key < kend && (!mask || mask[key]);
+    kf.load(kb, a.sk.n, key, ok, a.dh);
+    vf.load(vb, a.sv.n, key, ok, a.dh);
+  };
+  load(t_lo + wave);
+  const int r = l & 31, g = r / a.Nq, n = r - g * a.Nq;
+  s16x8 qf[2 * HD];
+  const uint16_t* qp = a.q + b * a.sq.b + n * a.sq.n + (int64_t)(hk * a.G + g) * a.sq.h;
+#pragma unroll
+  for (int ks = 0; ks < 2 * HD; ++ks) qf[ks] = ld8(qp + ks * 16 + hi * 8, r < a.R && ks * 16 + hi * 8 < a.dh);
+  f32x16 o[HD];
+#pragma unroll
+  for (int db = 0; db < HD; ++db) o[db] = splat(0.f);
+  float m = M_NONE, lsum = 0.f;
+  const float c = a.scale * LOG2E;
+  for (int t = t_lo + wave; t < t_hi; t += 4) {
+    const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+    f32x16 s[1] = {splat(0.f)};
+    if (seen != 0xffffffffu) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[0][e] = (seen >> crow(e, hi)) & 1 ? 0.f : -INFINITY;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) s[0] = mma<F16>(kf.f[ks], qf[ks], s[0]);
+    vf.store_tr(img);
+    load(t + 4);
+    soft_step<HD, 1>(s, c, m, lsum, o);
+    const s16x8 p0 = pack8<F16>(s[0], 0), p1 = pack8<F16>(s[0], 8);
+    wait_lds();
+#pragma unroll
+    for (int db = 0; db < HD; ++db) {
+      o[db] = mma<F16>(tr_frag<HD>(img, db, 0), p0, o[db]);
+      o[db] = mma<F16>(tr_frag<HD>(img, db, 16), p1, o[db]);
+    }
+    wait_lds();
+  }
+  lsum = half_sum(lsum);
+  __syncthreads();   // the images become the waves' partial outputs
+  float* part = reinterpret_cast<float*>(smem) + wave * 32 * OST;
+  float2* ml = reinterpret_cast<float2*>(smem + 4 * 32 * OST * 4);
+  if (r < a.R) {
+    put_partial<HD>(part + r * OST, o, 1.f, HD * 32);
+    if (hi == 0) ml[wave * 32 + r] = make_float2(m, lsum);
+  }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(smem);
+  const int d4n = a.dh >> 2;
+  for (int i = threadIdx.x; i < a.R * d4n; i += NT) {
+    const int row = i / d4n, d = (i - row * d4n) * 4;
+    float mm = M_NONE, ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w * 32 + row].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f((ml[w * 32 + row].x - mm) * c);
+      const float4 x = *reinterpret_cast<const float4*>(all + (w * 32 + row) * OST + d);
+      ls += ml[w * 32 + row].y * f;
+      acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+    }
+    if (a.splits > 1) {
+      const int64_t rows = (int64_t)a.B * a.Hkv * a.R, at = split * rows + (int64_t)bh * a.R + row;
+      *reinterpret_cast<float4*>(a.ws + at * a.dh + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * a.dh + at * 2) = make_float2(mm, ls);
+    } else {
+      const int gg = row / a.Nq, nn = row - gg * a.Nq, h = hk * a.G + gg;
+      const float inv = ls != 0.f ? 1.f / ls : 0.f;
+      *reinterpret_cast<uint2*>(a.out + b * a.so.b + nn * a.so.n + h * a.so.h + d) =
+          make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
+      if (d == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + nn] = ls != 0.f ? mm * a.scale + __logf(ls) : -INFINITY;
+    }
+  }
+}
+
+// joins the key splits of the forward: per row the largest reference, the rescaled sums in split order
+template <bool F16>
+__global__ __launch_bounds__(NT) void xattn_join_kernel(const XArgs a) {
+  const int d4n = a.dh >> 2;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.R, i = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (i >= rows * d4n) return;
+  const int64_t row = i / d4n;
+  const int d = (int)(i - row * d4n) * 4, r = (int)(row % a.R);
+  const int64_t bh = row / a.R;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv), g = r / a.Nq, n = r - g * a.Nq, h = hk * a.G + g;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * rows * a.dh);
+  const float c = a.scale * LOG2E;
+  float mm = M_NONE, ls = 0.f;
+  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, ml[s * rows + row].x);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 y = ml[s * rows + row];
+    const float f = __builtin_amdgcn_exp2f((y.x - mm) * c);
+    const float4 x = *reinterpret_cast<const float4*>(a.ws + (s * rows + row) * a.dh + d);
+    ls += y.y * f;
+    acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
+  }
+  const float inv = ls != 0.f ? 1.f / ls : 0.f;
+  *reinterpret_cast<uint2*>(a.out + b * a.so.b + n * a.so.n + h * a.so.h + d) = make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
+  if (d == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + n] = ls != 0.f ? mm * a.scale + __logf(ls) : -INFINITY;
+}
+
+// ================================================================================================================== backward
+// The row statistics enter the products as accumulator start values: S' = S / scale - lse / scale, dP' = dP - D, so P = exp2(c S') and dS = P dP'.
+// A row without keys has lse = -inf: it starts at -inf like a row past the end, and every P is 0.
+__device__ __forceinline__ float row_start(float lse, float scale) { return lse == -INFINITY ? -INFINITY : -lse / scale; }
+
+// dQ: a workgroup owns 128 query rows and walks its share of the keys; D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
+template <bool F16, int HD>
+__global__ __launch_bounds__(NT) void xattn_dq_kernel(const XArgs a) {
+  constexpr int BUF = 2 * row_img<HD>() + tr_img<HD>() + KC * 4;
+  __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+  int bh, item;
+  if (!my_item(a, a.tiles * a.splits, bh, item)) return;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, split = item / a.tiles;
+  const int wave = threadIdx.x >> 6, l = lane(), hi = l >> 5;
+  const int kend = key_end(a, b), chunks = (kend + KC - 1) / KC, per = (chunks + a.splits - 1) / a.splits;
+  const int c_lo = min(split * per, chunks), c_hi = min(c_lo + per, chunks);
+  const uint16_t* kb = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
+  const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
+  Chunk<HD> kr, vr;
+  float bias = 0.f;
+  auto load = [&](int c) {
+    kr.load_keys(kb, a.sk.n, c * KC, kend, mask, a.dh);
+    vr.load_keys(vb, a.sv.n, c * KC, kend, mask, a.dh);
+    if (threadIdx.x < KC) { const int key = c * KC + threadIdx.x; bias = key < kend && (!mask || mask[key]) ? 0.f : -INFINITY; }
+  };
+  auto store = [&](int buf) {
+    char* p = smem + buf * BUF;
+    kr.store_rows(p);
+    vr.store_rows(p + row_img<HD>());
+    kr.store_tr(p + 2 * row_img<HD>());
+    if (threadIdx.x < KC) *reinterpret_cast<float*>(p + 2 * row_img<HD>() + tr_img<HD>() + threadIdx.x * 4) = bias;
+  };
+  if (c_lo < c_hi) load(c_lo);
+  const int row0 = (tile * 4 + wave) * 32, r = row0 + (l & 31), g = r / a.Nq, n = r - g * a.Nq;
+  const int64_t h = hk * a.G + g;
+  const float lse = r < a.R ? a.lse[((int64_t)b * a.H + h) * a.Nq + n] : -INFINITY;
+  const bool live = lse != -INFINITY;   // a row without keys takes no part: its dO may hold anything
+  s16x8 qf[2 * HD], df[2 * HD];
+  float D = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 2 * HD; ++ks) {
+    const int d = ks * 16 + hi * 8;
+    const bool ok = live && d < a.dh;
+    qf[ks] = ld8(a.q + b * a.sq.b + n * a.sq.n + h * a.sq.h + d, ok);
+    df[ks] = ld8(a.dout + b * a.sdo.b + n * a.sdo.n + h * a.sdo.h + d, ok);
+    const s16x8 of = ld8(a.o + b * a.so.b + n * a.so.n + h * a.so.h + d, ok);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) D = fmaf(to_f<F16>(df[ks][j]), to_f<F16>(of[j]), D);
+  }
+  D = half_sum(D);
+  if (split == 0 && hi == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = D;
+  const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
+  f32x16 dq[HD];
+#pragma unroll
+  for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
+  if (c_lo < c_hi) store(0);
+  __syncthreads();
+  for (int ch = c_lo; ch < c_hi; ++ch) {
+    const int buf = (ch - c_lo) & 1;
+    const bool more = ch + 1 < c_hi;
+    if (more) load(ch + 1);
+    const char* K = smem + buf * BUF;
+    const char* V = K + row_img<HD>();
+    const char* Kt = V + row_img<HD>();
+    const float* bs = reinterpret_cast<const float*>(Kt + tr_img<HD>());
+    if (row0 < a.R) {
+      const bool biased = mask || (ch + 1) * KC > kend;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16 s = splat(s0), dp = splat(-D);
+        if (biased) {
+#pragma unroll
+          for (int gq = 0; gq < 4; ++gq) {
+            const float4 x = *reinterpret_cast<const float4*>(bs + t * 32 + 8 * gq + 4 * hi);
+            s[4 * gq] += x.x; s[4 * gq + 1] += x.y; s[4 * gq + 2] += x.z; s[4 * gq + 3] += x.w;
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2 * HD; ++ks) {
+          s = mma<F16>(row_frag<HD>(K, t, ks), qf[ks], s);
+          dp = mma<F16>(row_frag<HD>(V, t, ks), df[ks], dp);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
+        const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
+#pragma unroll
+        for (int db = 0; db < HD; ++db) {
+          dq[db] = mma<F16>(tr_frag<HD>(Kt, db, t * 32), d0, dq[db]);
+          dq[db] = mma<F16>(tr_frag<HD>(Kt, db, t * 32 + 16), d1, dq[db]);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  if (r >= a.R) return;
+  if (a.splits > 1) put_partial<HD>(a.ws + ((int64_t)split * a.B * a.Hkv * a.R + (int64_t)bh * a.R + r) * a.dh, dq, a.scale, a.dh);
+  else put_row<F16, HD>(a.dq + b * a.sdq.b + n * a.sdq.n + h * a.sdq.h, dq, a.scale, a.dh);
+}
+
+// dK / dV: a wave owns 32 keys (K, V fragments and both accumulators in registers), the query rows pass through LDS in chunks of 64.
+template <bool F16, int HD>
+__global__ __launch_bounds__(NT) void xattn_dkdv_kernel(const XArgs a) {
+  constexpr int BUF = 2 * row_img<HD>() + 2 * tr_img<HD>() + 2 * KC * 4;
+  __shared__ __attribute__((aligned(16))) char smem[BUF];
+  int bh, item;
+  if (!my_item(a, a.tiles * a.splits, bh, item)) return;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, split = item / a.tiles;
+  const int wave = threadIdx.x >> 6, l = lane(), hi = l >> 5;
+  const int kend = key_end(a, b);
+  const int key = (tile * 4 + wave) * 32 + (l & 31);
+  const bool seen = key < kend && (!a.kmask || a.kmask[(int64_t)b * a.Nk + key]);
+  const int chunks = tile * 128 < kend ? (a.R + KC - 1) / KC : 0, per = (chunks + a.splits - 1) / a.splits;
+  const int c_lo = min(split * per, chunks), c_hi = min(c_lo + per, chunks);
+  const uint16_t* qb = a.q + b * a.sq.b + (int64_t)hk * a.G * a.sq.h;
+  const uint16_t* db_ = a.dout + b * a.sdo.b + (int64_t)hk * a.G * a.sdo.h;
+  Chunk<HD> qr, dr;
+  float l_reg = 0.f, d_reg = 0.f;
+  auto load = [&](int ch) {
+    qr.load_rows(qb, a.sq, ch * KC, a.R, a.Nq, a.dh);
+    dr.load_rows(db_, a.sdo, ch * KC, a.R, a.Nq, a.dh);
+    if (threadIdx.x < KC) {
+      const int r = ch * KC + threadIdx.x;
+      l_reg = r < a.R ? row_start(a.lse[((int64_t)b * a.H + hk * a.G) * a.Nq + r], a.scale) : -INFINITY;   // rows of a group lie one after the other
+      d_reg = r < a.R ? -a.delta[(int64_t)bh * a.R + r] : 0.f;
+    }
+  };
+  auto store = [&]() {
+    char* p = smem;
+    qr.store_rows(p); p += row_img<HD>();
+    dr.store_rows(p); p += row_img<HD>();
+    qr.store_tr(p); p += tr_img<HD>();
+    dr.store_tr(p); p += tr_img<HD>();
+    if (threadIdx.x < KC) {
+      reinterpret_cast<float*>(p)[threadIdx.x] = l_reg;
+      reinterpret_cast<float*>(p)[KC + threadIdx.x] = d_reg;
+    }
+  };
+  if (c_lo < c_hi) load(c_lo);
+  KeyTile<HD> kf, vf;
+  kf.load(a.k + b * a.sk.b + hk * a.sk.h, a.sk.n, key, seen, a.dh);
+  vf.load(a.v + b * a.sv.b + hk * a.sv.h, a.sv.n, key, seen, a.dh);
+  f32x16 dk[HD], dv[HD];
+#pragma unroll
+  for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
+  const float c = a.scale * LOG2E;
+  const bool any = __builtin_amdgcn_ballot_w64(seen) != 0;
+  for (int ch = c_lo; ch < c_hi; ++ch) {
+    if (ch > c_lo) __syncthreads();
+    store();
+    __syncthreads();
+    if (ch + 1 < c_hi) load(ch + 1);
+    if (!any) continue;
+    const char* Q = smem;
+    const char* O = Q + row_img<HD>();
+    const char* Qt = O + row_img<HD>();
+    const char* Ot = Qt + tr_img<HD>();
+    const float* st = reinterpret_cast<const float*>(Ot + tr_img<HD>());
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 x = *reinterpret_cast<const float4*>(st + t * 32 + 8 * g + 4 * hi);
+        const float4 y = *reinterpret_cast<const float4*>(st + KC + t * 32 + 8 * g + 4 * hi);
+        s[4 * g] = seen ? x.x : -INFINITY; s[4 * g + 1] = seen ? x.y : -INFINITY; s[4 * g + 2] = seen ? x.z : -INFINITY; s[4 * g + 3] = seen ? x.w : -INFINITY;
+        dp[4 * g] = y.x; dp[4 * g + 1] = y.y; dp[4 * g + 2] = y.z; dp[4 * g + 3] = y.w;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2 * HD; ++ks) {
+        s = mma<F16>(row_frag<HD>(Q, t, ks), kf.f[ks], s);
+        dp = mma<F16>(row_frag<HD>(O, t, ks), vf.f[ks], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(s[e] * c);
+        dp[e] *= p;
+        s[e] = F16 ? p * P_UP : p;
+      }
+      const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8), d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
+#pragma unroll
+      for (int db = 0; db < HD; ++db) {
+        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, t * 32), p0, dv[db]);
+        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, t * 32 + 16), p1, dv[db]);
+        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, t * 32), d0, dk[db]);
+        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, t * 32 + 16), d1, dk[db]);
+      }
+    }
+  }
+  if (key >= a.Nk) return;
+  if (!seen) {   // gradients of keys that are not visible are zero whatever dO holds
+#pragma unroll
+    for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
+  }
+  const float vmul = F16 ? 1.f / P_UP : 1.f;
+  if (a.splits > 1) {
+    const int64_t keys = (int64_t)a.B * a.Hkv * a.Nk, at = split * keys + (int64_t)bh * a.Nk + key;
+    put_partial<HD>(a.ws + at * a.dh, dk, a.scale, a.dh);
+    put_partial<HD>(a.ws + (a.splits * keys + at) * a.dh, dv, vmul, a.dh);
+  } else {
+    put_row<F16, HD>(a.dk + b * a.sdk.b + key * a.sdk.n + hk * a.sdk.h, dk, a.scale, a.dh);
+    put_row<F16, HD>(a.dv + b * a.sdv.b + key * a.sdv.n + hk * a.sdv.h, dv, vmul, a.dh);
+  }
+}
+
+// Few rows (R <= 32): every key tile meets the one row tile once, so dK / dV of the tile are complete at once and all three gradients take ONE pass
+// over K / V.  Each wave owns key tiles; S is formed in both orientations (lane -> key for dK / dV, lane -> query for dQ): the second set of
+// products costs less than turning dS through LDS, and the pass is bound by memory.
+template <bool F16, int HD>
+__global__ __launch_bounds__(NT) void xattn_bwd_few_kernel(const XArgs a) {
+  constexpr int IMG = 32 * HD * 64, OST = HD * 32 + 4;
+  constexpr int TAIL = 4 * 32 * OST * 4, HEAD = 6 * IMG + 2 * 32 * 4;
+  __shared__ __attribute__((aligned(16))) char smem[TAIL > HEAD ? TAIL : HEAD];
+  int bh, split;
+  if (!my_item(a, a.splits, bh, split)) return;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int wave = threadIdx.x >> 6, l = lane(), hi = l >> 5;
+  const int kend = key_end(a, b), tiles = (a.Nk + 31) / 32, per = (tiles + a.splits - 1) / a.splits;   // tiles behind kend: zeros to write
+  const int t_lo = min(split * per, tiles), t_hi = min(t_lo + per, tiles);
+  const uint16_t* kb = a.k + b * a.sk.b + hk * a.sk.h;
+  const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
+  const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
+  char* Qt = smem;
+  char* Ot = smem + IMG;
+  char* Kt = smem + (2 + wave) * IMG;
+  float* st = reinterpret_cast<float*>(smem + 6 * IMG);
+  KeyTile<HD> kn, vn;
+  bool okn = false;
+  auto load = [&](int t) {
+    const int key = t * 32 + (l & 31);
+    okn = t < t_hi && key < kend && (!mask || mask[key]);
+    kn.load(kb, a.sk.n, key, okn, a.dh);
+    vn.load(vb, a.sv.n, key, okn, a.dh);
+  };
+  load(t_lo + wave);
+  const int r = l & 31, g = r / a.Nq, n = r - g * a.Nq;
+  const int64_t h = hk * a.G + g;
+  const float lse = r < a.R ? a.lse[((int64_t)b * a.H + h) * a.Nq + n] : -INFINITY;
+  const bool live = lse != -INFINITY;
+  KeyTile<HD> q, d;
+  float D = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 2 * HD; ++ks) {
+    const int dd = ks * 16 + hi * 8;
+    const bool ok = live && dd < a.dh;
+    q.f[ks] = ld8(a.q + b * a.sq.b + n * a.sq.n + h * a.sq.h + dd, ok);
+    d.f[ks] = ld8(a.dout + b * a.sdo.b + n * a.sdo.n + h * a.sdo.h + dd, ok);
+    const s16x8 of = ld8(a.o + b * a.so.b + n * a.so.n + h * a.so.h + dd, ok);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) D = fmaf(to_f<F16>(d.f[ks][j]), to_f<F16>(of[j]), D);
+  }
+  D = half_sum(D);
+  const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
+  if (wave == 0) {
+    q.store_tr(Qt);
+    d.store_tr(Ot);
+    if (hi == 0) { st[r] = s0; st[32 + r] = -D; }
+  }
+  f32x16 dq[HD];
+#pragma unroll
+  for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
+  __syncthreads();
+  for (int t = t_lo + wave; t < t_hi; t += 4) {
+    const KeyTile<HD> kf = kn, vf = vn;
+    const bool seen = okn;
+    const uint32_t all = (uint32_t)__builtin_amdgcn_ballot_w64(seen);
+    load(t + 4);
+    kf.store_tr(Kt);
+    f32x16 dk[HD], dv[HD];
+    {
+      f32x16 s, dp;   // lane -> key
+#pragma unroll
+      for (int gq = 0; gq < 4; ++gq) {
+        const float4 x = *reinterpret_cast<const float4*>(st + 8 * gq + 4 * hi);
+        const float4 y = *reinterpret_cast<const float4*>(st + 32 + 8 * gq + 4 * hi);
+        s[4 * gq] = seen ? x.x : -INFINITY; s[4 * gq + 1] = seen ? x.y : -INFINITY; s[4 * gq + 2] = seen ? x.z : -INFINITY; s[4 * gq + 3] = seen ? x.w : -INFINITY;
+        dp[4 * gq] = y.x; dp[4 * gq + 1] = y.y; dp[4 * gq + 2] = y.z; dp[4 * gq + 3] = y.w;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2 * HD; ++ks) {
+        s = mma<F16>(q.f[ks], kf.f[ks], s);
+        dp = mma<F16>(d.f[ks], vf.f[ks], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(s[e] * c);
+        dp[e] *= p;
+        s[e] = F16 ? p * P_UP : p;
+      }
+      const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8), d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
+#pragma unroll
+      for (int db = 0; db < HD; ++db) {
+        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, 0), p0, splat(0.f));
+        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, 16), p1, dv[db]);
+        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, 0), d0, splat(0.f));
+        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, 16), d1, dk[db]);
+      }
+    }
+    const int key = t * 32 + (l & 31);
+    if (key < a.Nk) {
+      if (!seen) {
+#pragma unroll
+        for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
+      }
+      put_row<F16, HD>(a.dk + b * a.sdk.b + key * a.sdk.n + hk * a.sdk.h, dk, a.scale, a.dh);
+      put_row<F16, HD>(a.dv + b * a.sdv.b + key * a.sdv.n + hk * a.sdv.h, dv, F16 ? 1.f / P_UP : 1.f, a.dh);
+    }
+    f32x16 s = splat(s0), dp = splat(-D);   // lane -> query
+    if (all != 0xffffffffu) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = (all >> crow(e, hi)) & 1 ? s[e] : -INFINITY;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) {
+      s = mma<F16>(kf.f[ks], q.f[ks], s);
+      dp = mma<F16>(vf.f[ks], d.f[ks], dp);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
+    const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
+    wait_lds();
+#pragma unroll
+    for (int db = 0; db < HD; ++db) {
+      dq[db] = mma<F16>(tr_frag<HD>(Kt, db, 0), d0, dq[db]);
+      dq[db] = mma<F16>(tr_frag<HD>(Kt, db, 16), d1, dq[db]);
+    }
+    wait_lds();
+  }
+  __syncthreads();   // images -> the waves' partial dQ rows
+  if (r < a.R) put_partial<HD>(reinterpret_cast<float*>(smem) + (wave * 32 + r) * OST, dq, a.scale, HD * 32);
+  __syncthreads();
+  const float* part = reinterpret_cast<const float*>(smem);
+  const int d4n = a.dh >> 2;
+  for (int i = threadIdx.x; i < a.R * d4n; i += NT) {
+    const int row = i / d4n, dd = (i - row * d4n) * 4;
+    float4 acc = *reinterpret_cast<const float4*>(part + row * OST + dd);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(part + (w * 32 + row) * OST + dd);
+      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    }
+    if (a.splits > 1) {
+      *reinterpret_cast<float4*>(a.ws + ((int64_t)split * a.B * a.Hkv * a.R + (int64_t)bh * a.R + row) * a.dh + dd) = acc;
+    } else {
+      const int gg = row / a.Nq, nn = row - gg * a.Nq;
+      *reinterpret_cast<uint2*>(a.dq + b * a.sdq.b + nn * a.sdq.n + (int64_t)(hk * a.G + gg) * a.sdq.h + dd) = make_uint2(pack2<F16>(acc.x, acc.y), pack2<F16>(acc.z, acc.w));
+    }
+  }
+}
+
+// adds the splits' partial rows in split order: row (bh, r) of `part` [splits][B * Hkv * R][dh] -> dst rows of head hk * G + r / Nq, token r % Nq
+template <bool F16>
+__global__ __launch_bounds__(NT) void xattn_add_kernel(const float* __restrict__ part, uint16_t* __restrict__ dst, Strides s, int splits, int64_t rows, int R,
+                                                       int Nq, int G, int Hkv, int dh) {
+  const int d4n = dh >> 2;
+  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (i >= rows * d4n) return;
+  const int64_t row = i / d4n;
+  const int d = (int)(i - row * d4n) * 4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < splits; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(part + (k * rows + row) * dh + d);
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  }
+  const int64_t bh = row / R;
+  const int r = (int)(row - bh * R), g = r / Nq, n = r - g * Nq;
+  const int64_t b = bh / Hkv, h = (bh % Hkv) * G + g;
+  *reinterpret_cast<uint2*>(dst + b * s.b + n * s.n + h * s.h + d) = make_uint2(pack2<F16>(acc.x, acc.y), pack2<F16>(acc.z, acc.w));
+}
+
+// ================================================================================================================== host
+constexpr int CUS = 256;
+struct Plan { bool few; int tiles, splits; };
+
+int round_up8(int64_t x) { return (int)((x + 7) / 8 * 8); }
+
+// `blocks` workgroups without a split along an axis of `chunks` pieces: split until the card has about `want` workgroups, with at least `least`
+// pieces left to each
+int split_for(int64_t blocks, int chunks, int want, int least) {
+  if (blocks <= 0 || blocks >= want || chunks < 2 * least) return 1;
+  int64_t s = (want + blocks - 1) / blocks;
+  if (s > chunks / least) s = chunks / least;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : (int)s;
+}
+bool few_rows(int R) { return R <= 32; }
+int row_tiles(int HD) { return HD <= 2 ? 2 : 1; }   // 32-row tiles per wave of the tiled forward
+
+Plan fwd_plan(int B, int R, int Nk, int Hkv, int dh) {
+  const int64_t bh = (int64_t)B * Hkv;
+  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 32), 3 * CUS, 8)};
+  const int tiles = lt_cdiv(R, 128 * row_tiles(lt_cdiv(dh, 32)));
+  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), 2 * CUS, 4)};
+}
+Plan dq_plan(int B, int R, int Nk, int Hkv) {
+  const int64_t bh = (int64_t)B * Hkv;
+  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 32), 3 * CUS, 4)};
+  const int tiles = lt_cdiv(R, 128);
+  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), 2 * CUS, 4)};
+}
+Plan dkdv_plan(int B, int R, int Nk, int Hkv) {
+  const int tiles = lt_cdiv(Nk, 128);
+  return {false, tiles, split_for((int64_t)B * Hkv * tiles, lt_cdiv(R, KC), 2 * CUS, 4)};
+}
+int64_t fwd_floats(int B, int R, int Nk, int Hkv, int dh) {
+  const Plan p = fwd_plan(B, R, Nk, Hkv, dh);
+  return p.splits > 1 ? (int64_t)p.splits * B * Hkv * R * (dh + 2) : 0;
+}
+int64_t dq_floats(int B, int R, int Nk, int Hkv, int dh) {
+  const Plan p = dq_plan(B, R, Nk, Hkv);
+  return p.splits > 1 ? (int64_t)p.splits * B * Hkv * R * dh : 0;
+}
+int64_t delta_floats(int B, int R, int Hkv) { return ((int64_t)B * Hkv * R + 3) / 4 * 4; }
+int64_t bwd_floats(int B, int R, int Nk, int Hkv, int dh) {
+  int64_t n = dq_floats(B, R, Nk, Hkv, dh);
+  if (few_rows(R)) return n;
+  const Plan p = dkdv_plan(B, R, Nk, Hkv);
+  const int64_t kv = p.splits > 1 ? 2 * (int64_t)p.splits * B * Hkv * Nk * dh : 0;
+  return delta_floats(B, R, Hkv) + (n > kv ? n : kv);
+}
+
+bool strides_ok(const int64_t* s, int B, int N, int H) {
+  return (B == 1 || (s[0] >= 0 && s[0] % 8 == 0)) && (N == 1 || (s[1] >= 0 && s[1] % 8 == 0)) && (H == 1 || (s[2] >= 0 && s[2] % 8 == 0));
+}
+Strides st3(const int64_t* s) { return {s[0], s[1], s[2]}; }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
+  LT_CHECK_ARG(d->B >= 0 && d->Nq >= 0 && d->Nk >= 0 && d->H > 0 && d->Hkv > 0 && d->H % d->Hkv == 0, "%s: bad sizes (B %d, Nq %d, Nk %d, H %d, Hkv %d)", who, d->B,
+               d->Nq, d->Nk, d->H, d->Hkv);
+  LT_CHECK_ARG(d->dh >= 8 && d->dh <= 128 && d->dh % 8 == 0, "%s: head_dim must be a multiple of 8 from 8 to 128 (got %d)", who, d->dh);
+  LT_CHECK_ARG(d->dtype == LT_DT_BF16 || d->dtype == LT_DT_F16, "%s: dtype must be LT_DT_BF16 or LT_DT_F16", who);
+  LT_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
+  LT_CHECK_ARG((int64_t)d->Nq * (d->H / d->Hkv) < (1 << 24) && d->Nk < (1 << 24) && (int64_t)d->B * d->Hkv < (1 << 20), "%s: sizes out of range", who);
+  const int G = d->H / d->Hkv;
+  if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->q && aligned16(d->q) && strides_ok(d->sq, d->B, d->Nq, d->H), "%s: q: 16-byte alignment of the pointer and of every stride", who);
+  if (d->Nk > 0 && d->B > 0)
+    LT_CHECK_ARG(d->k && d->v && aligned16(d->k) && aligned16(d->v) && strides_ok(d->sk, d->B, d->Nk, d->Hkv) && strides_ok(d->sv, d->B, d->Nk, d->Hkv),
+                 "%s: k, v: 16-byte alignment of the pointers and of every stride", who);
+  if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->out && aligned16(d->out) && strides_ok(d->so, d->B, d->Nq, d->H), "%s: out: 16-byte alignment of the pointer and of every stride", who);
+  a = XArgs{};
+  a.q = (const uint16_t*)d->q; a.k = (const uint16_t*)d->k; a.v = (const uint16_t*)d->v;
+  a.o = (const uint16_t*)d->out; a.out = (uint16_t*)d->out; a.lse = d->lse;
+  a.klen = d->key_lens; a.kmask = d->key_mask;
+  a.sq = st3(d->sq); a.sk = st3(d->sk); a.sv = st3(d->sv); a.so = st3(d->so);
+  a.B = d->B; a.Nq = d->Nq; a.Nk = d->Nk; a.H = d->H; a.Hkv = d->Hkv; a.G = G; a.R = G * d->Nq; a.dh = d->dh; a.scale = d->scale;
+  return LT_OK;
+}
+
+#define XA_HD(KERNEL, GRID, F16, ...)                                                                                    \
+  switch (lt_cdiv(a.dh, 32)) {                                                                                           \
+    case 1: hipLaunchKernelGGL((KERNEL<F16, 1 __VA_ARGS__>), dim3(GRID), dim3(NT), 0, (hipStream_t)stream, a); break;    \
+    case 2: hipLaunchKernelGGL((KERNEL<F16, 2 __VA_ARGS__>), dim3(GRID), dim3(NT), 0, (hipStream_t)stream, a); break;    \
+    case 3: hipLaunchKernelGGL((KERNEL<F16, 3 __VA_ARGS__>), dim3(GRID), dim3(NT), 0, (hipStream_t)stream, a); break;    \
+    default: hipLaunchKernelGGL((KERNEL<F16, 4 __VA_ARGS__>), dim3(GRID), dim3(NT), 0, (hipStream_t)stream, a); break;   \
+  }
+
+template <bool F16> void run_fwd(const XArgs& a, bool few, void* stream) {
+  const int64_t items = (int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits;
+  if (few) { XA_HD(xattn_fwd_few_kernel, (unsigned)items, F16) }
+  else {
+    switch (lt_cdiv(a.dh, 32)) {
+      case 1: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 1, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
+      case 2: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 2, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
+      case 3: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 3, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
+      default: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 4, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
+    }
+  }
+  if (a.splits > 1) {
+    const int64_t n = (int64_t)a.B * a.Hkv * a.R * (a.dh / 4);
+    hipLaunchKernelGGL(xattn_join_kernel<F16>, dim3((unsigned)lt_cdiv(n, NT)), dim3(NT), 0, (hipStream_t)stream, a);
+  }
+}
+template <bool F16> void add_splits(const XArgs& a, const float* part, uint16_t* dst, Strides s, int64_t rows, int R, int Nq, int G, void* stream) {
+  hipLaunchKernelGGL(xattn_add_kernel<F16>, dim3((unsigned)lt_cdiv(rows * (a.dh / 4), NT)), dim3(NT), 0, (hipStream_t)stream, part, dst, s, a.splits, rows, R, Nq, G,
+                     a.Hkv, a.dh);
+}
+template <bool F16> void run_bwd(XArgs a, float* ws, void* stream) {
+  const int64_t bh8 = round_up8((int64_t)a.B * a.Hkv), rows = (int64_t)a.B * a.Hkv * a.R, keys = (int64_t)a.B * a.Hkv * a.Nk;
+  Plan p = dq_plan(a.B, a.R, a.Nk, a.Hkv);
+  a.tiles = p.tiles; a.splits = p.splits;
+  a.delta = ws;
+  a.ws = p.few ? ws : ws + delta_floats(a.B, a.R, a.Hkv);
+  if (p.few) { XA_HD(xattn_bwd_few_kernel, (unsigned)(bh8 * a.splits), F16) }
+  else { XA_HD(xattn_dq_kernel, (unsigned)(bh8 * a.tiles * a.splits), F16) }
+  if (a.splits > 1) add_splits<F16>(a, a.ws, a.dq, a.sdq, rows, a.R, a.Nq, a.G, stream);
+  if (p.few || a.Nk == 0) return;
+  p = dkdv_plan(a.B, a.R, a.Nk, a.Hkv);
+  a.tiles = p.tiles; a.splits = p.splits;
+  XA_HD(xattn_dkdv_kernel, (unsigned)(bh8 * a.tiles * a.splits), F16)
+  if (a.splits > 1) {
+    add_splits<F16>(a, a.ws, a.dk, a.sdk, keys, a.Nk, a.Nk, 1, stream);
+    add_splits<F16>(a, a.ws + a.splits * keys * a.dh, a.dv, a.sdv, keys, a.Nk, a.Nk, 1, stream);
+  }
+}
+
+__global__ void xattn_zero_kernel(uint16_t* dst, Strides s, int64_t n, int N, int H, int d8) {
+  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (i >= n) return;
+  const int c = (int)(i % d8), h = (int)(i / d8 % H);
+  const int64_t t = i / d8 / H;
+  *reinterpret_cast<uint4*>(dst + t / N * s.b + t % N * s.n + h * s.h + c * 8) = make_uint4(0, 0, 0, 0);
+}
+
+}  // namespace
+
+extern "C" int64_t lt_cross_attention_fwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh) {
+  if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 128) return 0;
+  return fwd_floats(B, Nq * (H / Hkv), Nk, Hkv, dh);
+}
+extern "C" int64_t lt_cross_attention_bwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh) {
+  if (B <= 0 || Nq <= 0 || Nk < 0 || H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 128) return 0;
+  return bwd_floats(B, Nq * (H / Hkv), Nk, Hkv, dh);
+}
+
+extern "C" int lt_cross_attention_fwd(const lt_cross_attention_desc* d, void* stream) {
+  LT_CHECK_ARG(d, "lt_cross_attention_fwd: no descriptor");
+  XArgs a;
+  const int rc = fill(d, a, "lt_cross_attention_fwd");
+  if (rc != LT_OK) return rc;
+  if (d->B == 0 || d->Nq == 0) return LT_OK;
+  const Plan p = fwd_plan(a.B, a.R, a.Nk, a.Hkv, a.dh);
+  a.tiles = p.tiles; a.splits = p.splits; a.ws = d->ws;
+  const int64_t need = fwd_floats(a.B, a.R, a.Nk, a.Hkv, a.dh);
+  LT_CHECK_ARG(need == 0 || (d->ws && aligned16(d->ws) && d->ws_floats >= need), "lt_cross_attention_fwd: a workspace of %lld floats is needed (got %lld)", (long long)need,
+               (long long)(d->ws ? d->ws_floats : 0));
+  LT_CHECK_ARG((int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits < (1ll << 31), "lt_cross_attention_fwd: too many workgroups");
+  if (d->dtype == LT_DT_F16) run_fwd<true>(a, p.few, stream);
+  else run_fwd<false>(a, p.few, stream);
+  LT_CHECK_LAUNCH("lt_cross_attention_fwd");
+}
+
+extern "C" int lt_cross_attention_bwd(const lt_cross_attention_desc* d, void* stream) {
+  LT_CHECK_ARG(d, "lt_cross_attention_bwd: no descriptor");
+  XArgs a;
+  const int rc = fill(d, a, "lt_cross_attention_bwd");
+  if (rc != LT_OK) return rc;
+  if (d->B == 0) return LT_OK;
+  if (d->Nq > 0)
+    LT_CHECK_ARG(d->lse && d->dout && d->dq && aligned16(d->dout) && aligned16(d->dq) && strides_ok(d->sdo, d->B, d->Nq, d->H) && strides_ok(d->sdq, d->B, d->Nq, d->H),
+                 "lt_cross_attention_bwd: lse, dout, dq: missing, or pointer or strides not 16-byte aligned");
+  if (d->Nk > 0)
+    LT_CHECK_ARG(d->dk && d->dv && aligned16(d->dk) && aligned16(d->dv) && strides_ok(d->sdk, d->B, d->Nk, d->Hkv) && strides_ok(d->sdv, d->B, d->Nk, d->Hkv),
+                 "lt_cross_attention_bwd: dk, dv: missing, or pointer or strides not 16-byte aligned");
+  a.dout = (const uint16_t*)d->dout; a.dq = (uint16_t*)d->dq; a.dk = (uint16_t*)d->dk; a.dv = (uint16_t*)d->dv;
+  a.sdo = st3(d->sdo); a.sdq = st3(d->sdq); a.sdk = st3(d->sdk); a.sdv = st3(d->sdv);
+  if (d->Nq == 0) {   // no queries: the keys' gradients are zero
+    if (d->Nk > 0) {
+      const int64_t n = (int64_t)a.B * a.Nk * a.Hkv * (a.dh / 8);
+      hipLaunchKernelGGL(xattn_zero_kernel, dim3((unsigned)lt_cdiv(n, NT)), dim3(NT), 0, (hipStream_t)stream, a.dk, a.sdk, n, a.Nk, a.Hkv, a.dh / 8);
+      hipLaunchKernelGGL(xattn_zero_kernel, dim3((unsigned)lt_cdiv(n, NT)), dim3(NT), 0, (hipStream_t)stream, a.dv, a.sdv, n, a.Nk, a.Hkv, a.dh / 8);
+    }
+    LT_CHECK_LAUNCH("lt_cross_attention_bwd");
+  }
+  const int64_t need = bwd_floats(a.B, a.R, a.Nk, a.Hkv, a.dh);
+  LT_CHECK_ARG(need == 0 || (d->ws && aligned16(d->ws) && d->ws_floats >= need), "lt_cross_attention_bwd: a workspace of %lld floats is needed (got %lld)", (long long)need,
+               (long long)(d->ws ? d->ws_floats : 0));
+  const int64_t bh8 = round_up8((int64_t)a.B * a.Hkv);
+  const Plan p1 = dq_plan(a.B, a.R, a.Nk, a.Hkv), p2 = dkdv_plan(a.B, a.R, a.Nk, a.Hkv);
+  LT_CHECK_ARG(bh8 * p1.tiles * p1.splits < (1ll << 31) && bh8 * p2.tiles * p2.splits < (1ll << 31), "lt_cross_attention_bwd: too many workgroups");
+  if (d->dtype == LT_DT_F16) run_bwd<true>(a, d->ws, stream);
+  else run_bwd<false>(a, d->ws, stream);
+  LT_CHECK_LAUNCH("lt_cross_attention_bwd");
+}

@@ -10,7 +10,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import (EPI_BF16, EPI_BF16_GELU, EPI_BF16_GELUGRAD, EPI_F32, EPI_F32_ACCUM, EPI_RESID, GemmDesc, check)
+from ._lib import (CrossAttentionDesc, EPI_BF16, EPI_BF16_GELU, EPI_BF16_GELUGRAD, EPI_F32, EPI_F32_ACCUM, EPI_RESID, GemmDesc, check)
 
 __all__ = ["EPI_BF16", "EPI_BF16_GELU", "EPI_RESID", "EPI_F32", "EPI_BF16_GELUGRAD", "EPI_F32_ACCUM"]
 
@@ -45,7 +45,7 @@ def _chk(t: Tensor, dtype: torch.dtype, name: str) -> None:
 # profiles/r05_graph_replay_ab.log) a replay issues the very same launches on the very same streams as the eager step: the device sees
 # no difference, results are bitwise equal by construction, and the library's host-side state (reduction ledger) runs as it does eagerly.
 _QUERY_CALLS = frozenset(("lt_last_error", "lt_abi_version", "lt_device_info", "lt_attention_bwd_ws_floats", "lt_batchnorm_ws_floats",
-                          "lt_reduce_overflows"))
+                          "lt_reduce_overflows", "lt_cross_attention_fwd_ws_floats", "lt_cross_attention_bwd_ws_floats"))
 _EV_RECORD, _EV_WAIT = torch.cuda.Event.record, torch.cuda.Event.wait
 
 
@@ -556,6 +556,114 @@ def attention_bwd(qkv: Tensor, out: Tensor, dout: Tensor, lse: Tensor, ws: Tenso
     assert ws.numel() >= attention_bwd_ws_floats(B, N, H, dh)
     check(_lib.load().lt_attention_bwd(_p(qkv), _p(out), _p(dout), _p(lse), _p(ws), _p(dqkv), B, N, H, dh, scale, _stream()),
           "lt_attention_bwd")
+
+
+_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # LT_DT_*
+
+
+def _here(t: Tensor, name: str) -> None:
+    """The launch goes to the current device's current stream: the tensor has to live on that device."""
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected a tensor on the current device (cuda:{torch.cuda.current_device() if torch.cuda.is_available() else '-'}), got {t.device}")
+
+
+def _strided(t: Tensor, shape: tuple, dtype: torch.dtype, name: str, out: bool = False) -> Tensor:
+    """A [batch, token, head, d] view that the strided kernels can read (or write) in place."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
+    _here(t, name)
+    step = 16 // t.element_size()
+    st = t.stride()
+    if t.numel() and (st[3] != 1 or t.data_ptr() % 16 or any(n > 1 and s % step for n, s in zip(shape[:3], st))):
+        raise ValueError(f"{name}: the last dimension must be contiguous, the pointer and the other strides multiples of 16 bytes (strides {st})")
+    if out and any(n > 1 and s == 0 for n, s in zip(shape[:3], st)):
+        raise ValueError(f"{name}: an output must not be a broadcast view (strides {st})")
+    return t
+
+
+def _flat(t: Optional[Tensor], shape: tuple, dtypes: tuple, name: str) -> Optional[Tensor]:
+    if t is None:
+        return None
+    if t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous {' / '.join(str(x) for x in dtypes)} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}, "
+                         f"contiguous={t.is_contiguous()}")
+    _here(t, name)
+    return t
+
+
+def cross_attention_fwd_ws_floats(B: int, Nq: int, Nk: int, H: int, Hkv: int, dh: int) -> int:
+    return int(_lib.load().lt_cross_attention_fwd_ws_floats(B, Nq, Nk, H, Hkv, dh))
+
+
+def cross_attention_bwd_ws_floats(B: int, Nq: int, Nk: int, H: int, Hkv: int, dh: int) -> int:
+    return int(_lib.load().lt_cross_attention_bwd_ws_floats(B, Nq, Nk, H, Hkv, dh))
+
+
+def _xattn_desc(who: str, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optional[Tensor], scale: float, key_lens: Optional[Tensor],
+                key_mask: Optional[Tensor], ws: Optional[Tensor], ws_floats: Any, written: bool) -> CrossAttentionDesc:
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"{who}: q, k, v are [batch, token, head, d] views, got {tuple(q.shape)} and {tuple(k.shape)}")
+    B, Nq, H, dh = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{who}: q must be bfloat16 or float16, got {q.dtype}")
+    if Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"{who}: the query heads ({H}) must be a multiple of the key heads ({Hkv})")
+    if dh % 8 or not 8 <= dh <= 128:
+        raise ValueError(f"{who}: head_dim must be a multiple of 8 from 8 to 128, got {dh}")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"{who}: scale must be positive and finite, got {scale}")
+    dt = q.dtype
+    _strided(q, (B, Nq, H, dh), dt, who + ".q")
+    _strided(k, (B, Nk, Hkv, dh), dt, who + ".k")
+    _strided(v, (B, Nk, Hkv, dh), dt, who + ".v")
+    _strided(out, (B, Nq, H, dh), dt, who + ".out", written)
+    _flat(lse, (B, H, Nq), (torch.float32,), who + ".lse")
+    _flat(key_lens, (B,), (torch.int32,), who + ".key_lens")
+    _flat(key_mask, (B, Nk), (torch.bool, torch.uint8), who + ".key_mask")
+    need = ws_floats(B, Nq, Nk, H, Hkv, dh)
+    if ws is None:
+        ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
+    elif ws.dtype != torch.float32 or not ws.is_contiguous() or ws.numel() < need:
+        raise ValueError(f"{who}.ws: expected at least {need} contiguous float32, got {ws.numel()} of {ws.dtype}")
+    else:
+        _here(ws, who + ".ws")
+    d = CrossAttentionDesc()
+    d.B, d.Nq, d.Nk, d.H, d.Hkv, d.dh, d.dtype, d.scale = B, Nq, Nk, H, Hkv, dh, _DT[dt], scale
+    d.q, d.k, d.v, d.out, d.lse, d.key_lens, d.key_mask = _p(q), _p(k), _p(v), _p(out), _p(lse), _p(key_lens), _p(key_mask)
+    d.sq[:], d.sk[:], d.sv[:], d.so[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3]
+    d.ws, d.ws_floats = _p(ws), (ws.numel() if ws is not None else 0)
+    d._keep = ws      # (a workspace made here lives as long as the descriptor, i.e. as a recorded launch)
+    return d
+
+
+def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optional[Tensor], scale: float, key_lens: Optional[Tensor] = None,
+                        key_mask: Optional[Tensor] = None, ws: Optional[Tensor] = None) -> None:
+    """out = softmax(scale * q k^T) v for queries q [B, Nq, H, dh] against another sequence's k, v [B, Nk, Hkv, dh] (bf16 or f16, strided views
+    allowed, H a multiple of Hkv); lse f32 [B, H, Nq] (needed by the backward) or None.  key_lens int32 [B], key_mask bool / uint8 [B, Nk]: which keys
+    are visible; a row without one gives out = 0, lse = -inf.  ws: f32 scratch of `cross_attention_fwd_ws_floats` elements, allocated
+    here when None; calls that may run at the same time need their own (lt_cross_attention_fwd)."""
+    d = _xattn_desc("cross_attention_fwd", q, k, v, out, lse, scale, key_lens, key_mask, ws, cross_attention_fwd_ws_floats, True)
+    check(_lib.load().lt_cross_attention_fwd(C.byref(d), _stream()), "lt_cross_attention_fwd")
+
+
+def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tensor, lse: Tensor, dq: Tensor, dk: Tensor, dv: Tensor, scale: float,
+                        key_lens: Optional[Tensor] = None, key_mask: Optional[Tensor] = None, ws: Optional[Tensor] = None) -> None:
+    """dq, dk, dv (overwritten; strided views allowed) of `cross_attention_fwd` from its out and lse and the upstream gradient dout.  Gradients of
+    broadcast inputs (stride 0) come back per batch entry, those of shared key heads summed over the heads that read them; keys that are
+    not visible get zeros.  ws: f32 scratch of `cross_attention_bwd_ws_floats` elements (lt_cross_attention_bwd)."""
+    who = "cross_attention_bwd"
+    if lse is None:
+        raise ValueError(f"{who}.lse: the forward's lse is needed")
+    d = _xattn_desc(who, q, k, v, out, lse, scale, key_lens, key_mask, ws, cross_attention_bwd_ws_floats, False)
+    dt, sq, sk = q.dtype, tuple(q.shape), tuple(k.shape)
+    _strided(dout, sq, dt, who + ".dout")
+    _strided(dq, sq, dt, who + ".dq", True)
+    _strided(dk, sk, dt, who + ".dk", True)
+    _strided(dv, sk, dt, who + ".dv", True)
+    d.dout, d.dq, d.dk, d.dv = _p(dout), _p(dq), _p(dk), _p(dv)
+    d.sdo[:], d.sdq[:], d.sdk[:], d.sdv[:] = dout.stride()[:3], dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+    check(_lib.load().lt_cross_attention_bwd(C.byref(d), _stream()), "lt_cross_attention_bwd")
 
 
 # ------------------------------------------------------------------------------------------ head pieces
