@@ -110,6 +110,21 @@ int lt_im2col_bf16(const float* img, void* cols, int B, int C, int H, int W, int
 int lt_rope_apply(void* qkv_bf16, const float* sin_t, const float* cos_t, int B, int N, int H, int dh, int prefix, int inverse,
                   void* stream);
 
+/* Rotary positions with several axes (time, height, width: images and video), beside the two-axis table form above: pair i of a head turns by
+ * pos[token][axis[i]] * freqs[i] radians, the angle formed in 64 bits; inverse = 1 the transposed rotation (the gradient).  x [B, N, H, dh] -> out, and in
+ * the same launch x2 [B, N, H2, dh] -> out2 when H2 > 0 (q and k); out may be x (in place), any other overlap is not allowed.
+ *   pairs (i, i + dh / 2), or (2 i, 2 i + 1) when interleaved; axis[i] outside 0 .. axes - 1 or a token < prefix: passed through unchanged
+ *   pos [N - prefix, axes] (shared by the batch) or, pos_per_batch, [B, N - prefix, axes], int32 or (pos_float) f32; freqs f32, axis int32 [dh / 2]
+ *   dh 8 .. 256, a multiple of 8, last dimension contiguous; s?? = element strides of (batch, token, head), pointers and strides 16-byte aligned */
+enum { LT_DT_BF16 = 0, LT_DT_F16 = 1, LT_DT_F32 = 2 };
+typedef struct lt_rope_axes_desc {
+  const void* x; const void* x2; void* out; void* out2;
+  const void* pos; const float* freqs; const int32_t* axis;
+  int64_t sx[3], so[3], sx2[3], so2[3];
+  int B, N, H, H2, dh, dtype, prefix, axes, pos_per_batch, pos_float, interleaved, inverse;
+} lt_rope_axes_desc;
+int lt_rope_axes(const lt_rope_axes_desc* d, void* stream);
+
 /* SwiGLU FFN gate (reference layers/swiglu_ffn.py:31-35): x12 bf16 [rows, 2H] = [x1 | x2], out bf16 [rows, H] =
  * silu(x1) * x2.  Backward: d12 bf16 [rows, 2H] = [dh * x2 * silu'(x1) | dh * silu(x1)].  H % 8 == 0. */
 int lt_swiglu_fwd(const void* x12_bf16, void* out_bf16, int64_t rows, int H, void* stream);
@@ -222,7 +237,6 @@ int lt_attention_bwd(const void* qkv, const void* out_bf16, const void* dout_bf1
  *              calls that may run at the same time (other streams, other captured graphs) need their own
  * The backward needs out and lse as the forward left them.  Sums over workgroups are added in a fixed order: results are bitwise reproducible.
  * ------------------------------------------------------------------------------------------ */
-enum { LT_DT_BF16 = 0, LT_DT_F16 = 1, LT_DT_F32 = 2 };
 typedef struct lt_cross_attention_desc {
   const void* q; const void* k; const void* v;
   void* out;                      /* written by the forward, read by the backward */
@@ -290,6 +304,19 @@ int lt_ce_fwd_bwd_logits_bf16(const void* s_bf16, const void* t_logits_bf16, con
  * loss[0] += coef * KL, dlogits bf16 = coef/T * (softmax(s/T) - softmax(t/T)); rows `ld` (dlogits: `ldd`) elements apart */
 int lt_kl_fwd_bwd(const float* s_logits, const float* t_logits, int ld, float inv_temp, float coef, float* loss,
                   void* dlogits_bf16, int ldd, int rows, int K, void* stream);
+/* Distillation from a teacher's top logits, beside lt_kl_fwd_bwd (which needs the teacher's whole rows): the teacher is known on k entries
+ * (t_val, t_idx) per row of K classes.  Without t_lse the teacher's distribution is the softmax of the kept t_val * inv_temp; with t_lse [rows] = the
+ * log-sum-exp of the teacher's whole row times inv_temp, p_j = exp(t_val_j * inv_temp - t_lse) and all classes not kept are one bucket,
+ * p_rest = max(0, 1 - sum p) against the student's q_rest (no bucket where every class is kept).  q = softmax(s * inv_temp), w = coef * row_weight[r]:
+ *   loss_rows[r] = w * (sum_j p_j log(p_j / q_j) + p_rest log(p_rest / q_rest));  loss[0] += sum_r loss_rows[r] (loss may be NULL; order-fixed)
+ *   dlogits[r]   = w * inv_temp * (q_j - p_j on kept classes, q_i * (1 - p_rest / q_rest) elsewhere)       (dlogits may be NULL)
+ * An index outside 0 .. K - 1 is a missing entry; of an index that comes again in its row the first entry counts; a row without entries, of weight 0
+ * or (without t_lse) with all entries -inf gives loss 0 and gradient 0.
+ *   s rows ld apart, LT_DT_*; dlogits rows ldd apart, the type of s, or bf16 for f32 s; t_val LT_DT_* rows ldv apart; t_idx int32 or (idx_is_64)
+ *   int64 rows ldi apart; t_lse, row_weight f32 [rows] or NULL.  1 <= k <= 1024, k <= K <= 262144, inv_temp > 0 */
+int lt_topk_kl_fwd_bwd(const void* s, int s_dtype, int64_t ld, const void* t_val, int val_dtype, int64_t ldv, const void* t_idx, int idx_is_64, int64_t ldi,
+                       const float* t_lse, const float* row_weight, float inv_temp, float coef, float* loss_rows, float* loss, void* dlogits, int d_dtype,
+                       int64_t ldd, int rows, int K, int k, void* stream);
 /* g[b] = d[b] + d[b]^T for `batch` square bf16 matrices (n x n, row stride ld): upstream gradient of X X^T */
 int lt_symmetrize_bf16(const void* d, void* g, int batch, int n, int ld, void* stream);
 /* DistillationV3._mixup_data (distillationv3.py:356-368): out[b] = lam * x[b] + (1 - lam) * x[index[b]], index int64 [B] */

@@ -35,6 +35,15 @@ class CrossAttentionDesc(C.Structure):
     ]
 
 
+class RopeAxesDesc(C.Structure):
+    _fields_ = [
+        ("x", vp), ("x2", vp), ("out", vp), ("out2", vp), ("pos", vp), ("freqs", vp), ("axis", vp),
+        ("sx", i64 * 3), ("so", i64 * 3), ("sx2", i64 * 3), ("so2", i64 * 3),
+        ("B", i32), ("N", i32), ("H", i32), ("H2", i32), ("dh", i32), ("dtype", i32), ("prefix", i32), ("axes", i32), ("pos_per_batch", i32),
+        ("pos_float", i32), ("interleaved", i32), ("inverse", i32),
+    ]
+
+
 EPI_BF16, EPI_BF16_GELU, EPI_RESID, EPI_F32, EPI_BF16_GELUGRAD, EPI_F32_ACCUM = range(6)
 ABI_VERSION = 5   # lt_abi_version() of include/lt_amd.h this binding was written against
 
@@ -52,6 +61,8 @@ SIGNATURES: dict[str, list[Any]] = {
     "lt_mixup": [vp, vp, f32, vp, i32, i64, vp],
     "lt_resample_tokens": [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp],
     "lt_rope_apply": [vp, vp, vp, i32, i32, i32, i32, i32, i32, vp],
+    "lt_rope_axes": [C.POINTER(RopeAxesDesc), vp],
+    "lt_topk_kl_fwd_bwd": [vp, i32, i64, vp, i32, i64, vp, i32, i64, vp, vp, f32, f32, vp, vp, vp, i32, i64, i32, i32, i32, vp],
     "lt_gelu_fwd_bf16": [vp, vp, i64, vp],
     "lt_gelu_bwd_bf16": [vp, vp, vp, i64, vp],
     "lt_swiglu_fwd": [vp, vp, i64, i32, vp],

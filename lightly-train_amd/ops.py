@@ -10,7 +10,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import (CrossAttentionDesc, EPI_BF16, EPI_BF16_GELU, EPI_BF16_GELUGRAD, EPI_F32, EPI_F32_ACCUM, EPI_RESID, GemmDesc, check)
+from ._lib import (CrossAttentionDesc, EPI_BF16, EPI_BF16_GELU, EPI_BF16_GELUGRAD, EPI_F32, EPI_F32_ACCUM, EPI_RESID, GemmDesc, RopeAxesDesc, check)
 
 __all__ = ["EPI_BF16", "EPI_BF16_GELU", "EPI_RESID", "EPI_F32", "EPI_BF16_GELUGRAD", "EPI_F32_ACCUM"]
 
@@ -34,6 +34,39 @@ def _p(t: Optional[Tensor]) -> Optional[int]:
 def _chk(t: Tensor, dtype: torch.dtype, name: str) -> None:
     if t.dtype != dtype or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name}: expected contiguous device tensor of {dtype}, got {t.dtype} contiguous={t.is_contiguous()} cuda={t.is_cuda}")
+
+
+_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # LT_DT_*
+
+
+def _here(t: Tensor, name: str) -> None:
+    """The launch goes to the current device's current stream: the tensor has to live on that device."""
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name}: expected a tensor on the current device (cuda:{torch.cuda.current_device() if torch.cuda.is_available() else '-'}), got {t.device}")
+
+
+def _strided(t: Tensor, shape: tuple, dtype: torch.dtype, name: str, out: bool = False) -> Tensor:
+    """A [batch, token, head, d] view that the strided kernels can read (or write) in place."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
+    _here(t, name)
+    step = 16 // t.element_size()
+    st = t.stride()
+    if t.numel() and (st[3] != 1 or t.data_ptr() % 16 or any(n > 1 and s % step for n, s in zip(shape[:3], st))):
+        raise ValueError(f"{name}: the last dimension must be contiguous, the pointer and the other strides multiples of 16 bytes (strides {st})")
+    if out and any(n > 1 and s == 0 for n, s in zip(shape[:3], st)):
+        raise ValueError(f"{name}: an output must not be a broadcast view (strides {st})")
+    return t
+
+
+def _flat(t: Optional[Tensor], shape: tuple, dtypes: tuple, name: str) -> Optional[Tensor]:
+    if t is None:
+        return None
+    if t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous {' / '.join(str(x) for x in dtypes)} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}, "
+                         f"contiguous={t.is_contiguous()}")
+    _here(t, name)
+    return t
 
 
 # ------------------------------------------------------------------------------------------ launch plans
@@ -425,6 +458,39 @@ def kl_fwd_bwd(s_logits: Tensor, t_logits: Tensor, ld: int, inv_temp: float, coe
     check(_lib.load().lt_kl_fwd_bwd(_p(s_logits), _p(t_logits), ld, inv_temp, coef, _p(loss), _p(dlogits), ldd, rows, K, _stream()), "lt_kl_fwd_bwd")
 
 
+def topk_kl_fwd_bwd(s: Tensor, t_val: Tensor, t_idx: Tensor, inv_temp: float, coef: float, loss_rows: Tensor, dlogits: Optional[Tensor] = None,
+                    t_lse: Optional[Tensor] = None, row_weight: Optional[Tensor] = None, loss: Optional[Tensor] = None) -> None:
+    """KL divergence from a teacher known by k top logits a row (t_val bf16 / f16 / f32, t_idx int32 / int64, [rows, k]) to softmax(s * inv_temp), s [rows, K]
+    bf16 / f16 / f32: loss_rows f32 [rows] (overwritten), loss f32 [1] += their sum, dlogits [rows, K] (the type of s, or bf16 for f32 s).  t_lse f32 [rows]:
+    the log-sum-exp of the teacher's whole row * inv_temp; with it the classes not kept are one bucket, without it the kept logits are renormalised.  Index < 0
+    (or >= K): no entry; of a repeated index the first entry counts.  Row r is weighted by coef * row_weight[r] (lt_topk_kl_fwd_bwd)."""
+    who = "topk_kl_fwd_bwd"
+    if s.dim() != 2 or t_val.dim() != 2 or s.dtype not in _DT:
+        raise ValueError(f"{who}: s [rows, K] of bfloat16, float16 or float32 and t_val [rows, k], got {s.dtype} {tuple(s.shape)} and {tuple(t_val.shape)}")
+    rows, K = s.shape
+    k = t_val.shape[1]
+    if not 1 <= k <= min(K, 1024) or K > 262144:
+        raise ValueError(f"{who}: 1 <= k <= min(K, 1024) and K <= 262144, got k {k}, K {K}")
+    if not 0.0 < inv_temp < float("inf"):
+        raise ValueError(f"{who}: inv_temp must be positive and finite, got {inv_temp}")
+
+    def row_view(t: Tensor, n: int, dtypes: tuple, name: str) -> int:
+        if t.dtype not in dtypes or tuple(t.shape) != (rows, n) or (rows and n > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < n):
+            raise ValueError(f"{who}.{name}: expected {' / '.join(str(x) for x in dtypes)} [{rows}, {n}] with contiguous, separate rows, got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
+        _here(t, f"{who}.{name}")
+        return t.stride(0) if rows > 1 else n
+    ld = row_view(s, K, (s.dtype,), "s")
+    ldv = row_view(t_val, k, tuple(_DT), "t_val")
+    ldi = row_view(t_idx, k, (torch.int32, torch.int64), "t_idx")
+    ldd = row_view(dlogits, K, (s.dtype, torch.bfloat16) if s.dtype == torch.float32 else (s.dtype,), "dlogits") if dlogits is not None else 0
+    f32 = (torch.float32,)
+    _flat(loss_rows, (rows,), f32, who + ".loss_rows"); _flat(t_lse, (rows,), f32, who + ".t_lse"); _flat(row_weight, (rows,), f32, who + ".row_weight")
+    _flat(loss, (1,), f32, who + ".loss")
+    check(_lib.load().lt_topk_kl_fwd_bwd(_p(s), _DT[s.dtype], ld, _p(t_val), _DT[t_val.dtype], ldv, _p(t_idx), int(t_idx.dtype == torch.int64), ldi, _p(t_lse),
+                                         _p(row_weight), inv_temp, coef, _p(loss_rows), _p(loss), _p(dlogits), _DT[dlogits.dtype if dlogits is not None else s.dtype],
+                                         ldd, rows, K, k, _stream()), "lt_topk_kl_fwd_bwd")
+
+
 def symmetrize_bf16(d: Tensor, g: Tensor, batch: int, n: int, ld: int) -> None:
     _chk(d, torch.bfloat16, "symmetrize.d"); _chk(g, torch.bfloat16, "symmetrize.g")
     check(_lib.load().lt_symmetrize_bf16(_p(d), _p(g), batch, n, ld, _stream()), "lt_symmetrize_bf16")
@@ -497,6 +563,67 @@ def rope_apply(qkv: Tensor, sin_t: Tensor, cos_t: Tensor, B: int, N: int, H: int
     check(_lib.load().lt_rope_apply(_p(qkv), _p(sin_t), _p(cos_t), B, N, H, dh, prefix, int(inverse), _stream()), "lt_rope_apply")
 
 
+def rope_axes(x: Tensor, out: Tensor, pos: Tensor, freqs: Tensor, axis: Tensor, prefix: int = 0, interleaved: bool = False, inverse: bool = False,
+              x2: Optional[Tensor] = None, out2: Optional[Tensor] = None) -> None:
+    """Rotary positions with several axes: pair i of every head of x [B, N, H, dh] (bf16, f16 or f32, strided views allowed) turns by
+    pos[token, axis[i]] * freqs[i] into `out` (may be x); x2 [B, N, H2, dh] into out2 in the same launch (q and k).  pos int32 / f32
+    [N - prefix, axes] or, per sample, [B, N - prefix, axes], 1 to 4 axes; freqs f32 and axis int32 [dh / 2] (`rope_axes_tables`); tokens < prefix and pairs of an
+    axis outside the table pass through.  inverse: the transposed rotation, i.e. the gradient (lt_rope_axes)."""
+    who = "rope_axes"
+    if x.dim() != 4 or x.dtype not in _DT:
+        raise ValueError(f"{who}.x: expected a [batch, token, head, d] view of bfloat16, float16 or float32, got {x.dtype} of shape {tuple(x.shape)}")
+    B, N, H, dh = x.shape
+    if dh % 8 or not 8 <= dh <= 256:
+        raise ValueError(f"{who}: head_dim must be a multiple of 8 from 8 to 256, got {dh}")
+    if not 0 <= prefix <= N:
+        raise ValueError(f"{who}: prefix must lie between 0 and the {N} tokens, got {prefix}")
+    if (x2 is None) != (out2 is None):
+        raise ValueError(f"{who}: x2 and out2 come together")
+    dt, n = x.dtype, N - prefix
+    _strided(x, (B, N, H, dh), dt, who + ".x")
+    _strided(out, (B, N, H, dh), dt, who + ".out", True)
+    if pos.dim() not in (2, 3) or not 1 <= pos.shape[-1] <= 4:
+        raise ValueError(f"{who}.pos: expected [tokens, axes] or [batch, tokens, axes] with 1 to 4 axes, got {tuple(pos.shape)}")
+    A = pos.shape[-1]
+    _flat(pos, (n, A) if pos.dim() == 2 else (B, n, A), (torch.int32, torch.float32), who + ".pos")
+    _flat(freqs, (dh // 2,), (torch.float32,), who + ".freqs")
+    _flat(axis, (dh // 2,), (torch.int32,), who + ".axis")
+    d = RopeAxesDesc()
+    d.B, d.N, d.H, d.dh, d.dtype, d.prefix, d.axes = B, N, H, dh, _DT[dt], prefix, A
+    d.pos_per_batch, d.pos_float, d.interleaved, d.inverse = int(pos.dim() == 3), int(pos.dtype == torch.float32), int(interleaved), int(inverse)
+    d.x, d.out, d.pos, d.freqs, d.axis = _p(x), _p(out), _p(pos), _p(freqs), _p(axis)
+    d.sx[:], d.so[:] = x.stride()[:3], out.stride()[:3]
+    if x2 is not None:
+        if x2.dim() != 4:
+            raise ValueError(f"{who}.x2: expected a [batch, token, head, d] view, got shape {tuple(x2.shape)}")
+        d.H2 = x2.shape[2]
+        _strided(x2, (B, N, d.H2, dh), dt, who + ".x2")
+        _strided(out2, (B, N, d.H2, dh), dt, who + ".out2", True)
+        d.x2, d.out2 = _p(x2), _p(out2)
+        d.sx2[:], d.so2[:] = x2.stride()[:3], out2.stride()[:3]
+    check(_lib.load().lt_rope_axes(C.byref(d), _stream()), "lt_rope_axes")
+
+
+def rope_axes_tables(dh: int, pairs: Any, base: float = 10000.0, shared_spectrum: bool = False, device: Any = None) -> Any:
+    """(freqs f32, axis int32) [dh / 2] for `rope_axes`: `pairs[a]` consecutive rotary pairs belong to axis a, pairs left over are not rotated.  The
+    frequencies of an axis fall from 1 as base^(-i / pairs[a]), i its own count; shared_spectrum: as base^(-i / (dh / 2)) over all pairs of the head."""
+    half = dh // 2
+    if dh % 2 or not 1 <= len(pairs) <= 4 or any(n < 0 for n in pairs) or sum(pairs) > half:
+        raise ValueError(f"rope_axes_tables: 1 to 4 axes of together at most {half} pairs, got {list(pairs)}")
+    freqs, axis = torch.zeros(half, dtype=torch.float64), torch.full((half,), -1, dtype=torch.int32)
+    i = 0
+    for a, n in enumerate(pairs):
+        at = torch.arange(i, i + n, dtype=torch.float64) / half if shared_spectrum else torch.arange(n, dtype=torch.float64) / max(n, 1)
+        freqs[i:i + n], axis[i:i + n] = base ** -at, a
+        i += n
+    return freqs.float().to(device), axis.to(device)
+
+
+def rope_grid(*sizes: int, device: Any = None) -> Tensor:
+    """Positions int32 [prod(sizes), len(sizes)] of the cells of a grid, last axis fastest: `rope_grid(frames, rows, columns)` for video patch tokens."""
+    return torch.cartesian_prod(*[torch.arange(n, dtype=torch.int32) for n in sizes]).reshape(-1, len(sizes)).to(device)
+
+
 def gelu_fwd(x: Tensor, y: Tensor, n: int) -> Tensor:
     """y[:n] = gelu(x[:n]) on flat bf16 storage (erf form, nn.GELU())."""
     _chk(x, torch.bfloat16, "gelu_fwd.x")
@@ -556,39 +683,6 @@ def attention_bwd(qkv: Tensor, out: Tensor, dout: Tensor, lse: Tensor, ws: Tenso
     assert ws.numel() >= attention_bwd_ws_floats(B, N, H, dh)
     check(_lib.load().lt_attention_bwd(_p(qkv), _p(out), _p(dout), _p(lse), _p(ws), _p(dqkv), B, N, H, dh, scale, _stream()),
           "lt_attention_bwd")
-
-
-_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # LT_DT_*
-
-
-def _here(t: Tensor, name: str) -> None:
-    """The launch goes to the current device's current stream: the tensor has to live on that device."""
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name}: expected a tensor on the current device (cuda:{torch.cuda.current_device() if torch.cuda.is_available() else '-'}), got {t.device}")
-
-
-def _strided(t: Tensor, shape: tuple, dtype: torch.dtype, name: str, out: bool = False) -> Tensor:
-    """A [batch, token, head, d] view that the strided kernels can read (or write) in place."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
-    _here(t, name)
-    step = 16 // t.element_size()
-    st = t.stride()
-    if t.numel() and (st[3] != 1 or t.data_ptr() % 16 or any(n > 1 and s % step for n, s in zip(shape[:3], st))):
-        raise ValueError(f"{name}: the last dimension must be contiguous, the pointer and the other strides multiples of 16 bytes (strides {st})")
-    if out and any(n > 1 and s == 0 for n, s in zip(shape[:3], st)):
-        raise ValueError(f"{name}: an output must not be a broadcast view (strides {st})")
-    return t
-
-
-def _flat(t: Optional[Tensor], shape: tuple, dtypes: tuple, name: str) -> Optional[Tensor]:
-    if t is None:
-        return None
-    if t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: expected contiguous {' / '.join(str(x) for x in dtypes)} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}, "
-                         f"contiguous={t.is_contiguous()}")
-    _here(t, name)
-    return t
 
 
 def cross_attention_fwd_ws_floats(B: int, Nq: int, Nk: int, H: int, Hkv: int, dh: int) -> int:
