@@ -61,7 +61,7 @@ SIGNATURES: dict[str, list[Any]] = {
     "lt_mixup": [vp, vp, f32, vp, i32, i64, vp],
     "lt_resample_tokens": [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp],
     "lt_rope_apply": [vp, vp, vp, i32, i32, i32, i32, i32, i32, vp],
-    "lt_rope_axes": [C.POINTER(RopeAxesDesc), vp],
+    "lt_rope_axes": [vp, vp],
     "lt_topk_kl_fwd_bwd": [vp, i32, i64, vp, i32, i64, vp, i32, i64, vp, vp, f32, f32, vp, vp, vp, i32, i64, i32, i32, i32, vp],
     "lt_gelu_fwd_bf16": [vp, vp, i64, vp],
     "lt_gelu_bwd_bf16": [vp, vp, vp, i64, vp],
@@ -89,8 +89,8 @@ SIGNATURES: dict[str, list[Any]] = {
     "lt_attention_fwd": [vp, vp, vp, i32, i32, i32, i32, f32, vp],
     "lt_cross_attention_fwd_ws_floats": [i32, i32, i32, i32, i32, i32],
     "lt_cross_attention_bwd_ws_floats": [i32, i32, i32, i32, i32, i32],
-    "lt_cross_attention_fwd": [C.POINTER(CrossAttentionDesc), vp],
-    "lt_cross_attention_bwd": [C.POINTER(CrossAttentionDesc), vp],
+    "lt_cross_attention_fwd": [vp, vp],
+    "lt_cross_attention_bwd": [vp, vp],
     "lt_attention_bwd": [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp],
     "lt_l2norm_fwd": [vp, vp, vp, i32, i32, f32, vp],
     "lt_l2norm_bwd": [vp, vp, vp, vp, i32, i32, vp],

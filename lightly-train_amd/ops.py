@@ -3,14 +3,16 @@ allocations and the HIP stream; every arithmetic op below runs in liblt_amd.so."
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import struct
 from typing import Dict, Any, Any, Optional
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import (CrossAttentionDesc, EPI_BF16, EPI_BF16_GELU, EPI_BF16_GELUGRAD, EPI_F32, EPI_F32_ACCUM, EPI_RESID, GemmDesc, RopeAxesDesc, check)
+from ._lib import (EPI_BF16, EPI_BF16_GELU, EPI_BF16_GELUGRAD, EPI_F32, EPI_F32_ACCUM, EPI_RESID, GemmDesc, check)
 
 __all__ = ["EPI_BF16", "EPI_BF16_GELU", "EPI_RESID", "EPI_F32", "EPI_BF16_GELUGRAD", "EPI_F32_ACCUM"]
 
@@ -37,36 +39,53 @@ def _chk(t: Tensor, dtype: torch.dtype, name: str) -> None:
 
 
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # LT_DT_*
+_F32 = (torch.float32,)
+_NO_STRIDE = (0, 0, 0)
 
 
-def _here(t: Tensor, name: str) -> None:
-    """The launch goes to the current device's current stream: the tensor has to live on that device."""
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name}: expected a tensor on the current device (cuda:{torch.cuda.current_device() if torch.cuda.is_available() else '-'}), got {t.device}")
+def _device() -> int:
+    """The launch goes to the current device's current stream: the tensors have to live on that device (-1: there is none)."""
+    try:
+        return torch.cuda.current_device()
+    except (RuntimeError, AssertionError):
+        return -1
 
 
-def _strided(t: Tensor, shape: tuple, dtype: torch.dtype, name: str, out: bool = False) -> Tensor:
-    """A [batch, token, head, d] view that the strided kernels can read (or write) in place."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
-    _here(t, name)
-    step = 16 // t.element_size()
-    st = t.stride()
-    if t.numel() and (st[3] != 1 or t.data_ptr() % 16 or any(n > 1 and s % step for n, s in zip(shape[:3], st))):
-        raise ValueError(f"{name}: the last dimension must be contiguous, the pointer and the other strides multiples of 16 bytes (strides {st})")
-    if out and any(n > 1 and s == 0 for n, s in zip(shape[:3], st)):
-        raise ValueError(f"{name}: an output must not be a broadcast view (strides {st})")
-    return t
+def _elsewhere(t: Tensor, dev: int, name: str) -> ValueError:
+    return ValueError(f"{name}: expected a tensor on the current device ({f'cuda:{dev}' if dev >= 0 else 'there is none'}), got {t.device}")
 
 
-def _flat(t: Optional[Tensor], shape: tuple, dtypes: tuple, name: str) -> Optional[Tensor]:
+def _strided(t: Tensor, shape: Any, dtype: torch.dtype, dev: int, name: str, out: bool = False) -> tuple:
+    """Strides (batch, token, head) of a [batch, token, head, d] view that the strided kernels can read (or write) in place."""
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name}: expected {dtype} of shape {tuple(shape)}, got {t.dtype} of shape {tuple(t.shape)}")
+    if t.get_device() != dev or dev < 0:
+        raise _elsewhere(t, dev, name)
+    a, b, c, d = t.stride()
+    if (t.data_ptr() & 15 or d != 1 or (a | b | c) & (3 if dtype is torch.float32 else 7)) and t.numel():
+        step = 4 if dtype is torch.float32 else 8
+        if t.data_ptr() & 15 or (d != 1 and shape[3] > 1) or any(n > 1 and x % step for n, x in zip(shape, (a, b, c))):
+            raise ValueError(f"{name}: the last dimension must be contiguous, the pointer and the other strides multiples of 16 bytes (strides {t.stride()})")
+    if out and not (a and b and c) and any(n > 1 and x == 0 for n, x in zip(shape, (a, b, c))):
+        raise ValueError(f"{name}: an output must not be a broadcast view (strides {t.stride()})")
+    return a, b, c
+
+
+def _flat(t: Optional[Tensor], shape: tuple, dtypes: tuple, dev: int, name: str) -> int:
+    """Pointer of a contiguous tensor of that shape, 0 for None."""
     if t is None:
-        return None
-    if t.dtype not in dtypes or tuple(t.shape) != shape or not t.is_contiguous():
+        return 0
+    if t.dtype not in dtypes or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: expected contiguous {' / '.join(str(x) for x in dtypes)} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}, "
                          f"contiguous={t.is_contiguous()}")
-    _here(t, name)
-    return t
+    if t.get_device() != dev or dev < 0:
+        raise _elsewhere(t, dev, name)
+    return t.data_ptr()
+
+
+class _Desc(bytes):
+    """A packed descriptor; `keep`: a workspace made for this call, alive as long as a recorded launch of it."""
+    keep: Any = None
 
 
 # ------------------------------------------------------------------------------------------ launch plans
@@ -458,6 +477,19 @@ def kl_fwd_bwd(s_logits: Tensor, t_logits: Tensor, ld: int, inv_temp: float, coe
     check(_lib.load().lt_kl_fwd_bwd(_p(s_logits), _p(t_logits), ld, inv_temp, coef, _p(loss), _p(dlogits), ldd, rows, K, _stream()), "lt_kl_fwd_bwd")
 
 
+_INDEX, _F32_BF16 = (torch.int32, torch.int64), (torch.float32, torch.bfloat16)
+
+
+def _row_view(t: Tensor, rows: int, n: int, dtypes: tuple, dev: int, name: str) -> int:
+    """Row stride of a [rows, n] view with contiguous rows that do not overlap."""
+    a, b = t.stride() if t.dim() == 2 else (0, 0)
+    if t.dtype not in dtypes or t.shape != (rows, n) or (b != 1 and n > 1 and rows) or (rows > 1 and a < n):
+        raise ValueError(f"{name}: expected {' / '.join(str(x) for x in dtypes)} [{rows}, {n}] with contiguous, separate rows, got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
+    if t.get_device() != dev or dev < 0:
+        raise _elsewhere(t, dev, name)
+    return a if rows > 1 else n
+
+
 def topk_kl_fwd_bwd(s: Tensor, t_val: Tensor, t_idx: Tensor, inv_temp: float, coef: float, loss_rows: Tensor, dlogits: Optional[Tensor] = None,
                     t_lse: Optional[Tensor] = None, row_weight: Optional[Tensor] = None, loss: Optional[Tensor] = None) -> None:
     """KL divergence from a teacher known by k top logits a row (t_val bf16 / f16 / f32, t_idx int32 / int64, [rows, k]) to softmax(s * inv_temp), s [rows, K]
@@ -474,21 +506,20 @@ def topk_kl_fwd_bwd(s: Tensor, t_val: Tensor, t_idx: Tensor, inv_temp: float, co
     if not 0.0 < inv_temp < float("inf"):
         raise ValueError(f"{who}: inv_temp must be positive and finite, got {inv_temp}")
 
-    def row_view(t: Tensor, n: int, dtypes: tuple, name: str) -> int:
-        if t.dtype not in dtypes or tuple(t.shape) != (rows, n) or (rows and n > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < n):
-            raise ValueError(f"{who}.{name}: expected {' / '.join(str(x) for x in dtypes)} [{rows}, {n}] with contiguous, separate rows, got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
-        _here(t, f"{who}.{name}")
-        return t.stride(0) if rows > 1 else n
-    ld = row_view(s, K, (s.dtype,), "s")
-    ldv = row_view(t_val, k, tuple(_DT), "t_val")
-    ldi = row_view(t_idx, k, (torch.int32, torch.int64), "t_idx")
-    ldd = row_view(dlogits, K, (s.dtype, torch.bfloat16) if s.dtype == torch.float32 else (s.dtype,), "dlogits") if dlogits is not None else 0
-    f32 = (torch.float32,)
-    _flat(loss_rows, (rows,), f32, who + ".loss_rows"); _flat(t_lse, (rows,), f32, who + ".t_lse"); _flat(row_weight, (rows,), f32, who + ".row_weight")
-    _flat(loss, (1,), f32, who + ".loss")
-    check(_lib.load().lt_topk_kl_fwd_bwd(_p(s), _DT[s.dtype], ld, _p(t_val), _DT[t_val.dtype], ldv, _p(t_idx), int(t_idx.dtype == torch.int64), ldi, _p(t_lse),
-                                         _p(row_weight), inv_temp, coef, _p(loss_rows), _p(loss), _p(dlogits), _DT[dlogits.dtype if dlogits is not None else s.dtype],
-                                         ldd, rows, K, k, _stream()), "lt_topk_kl_fwd_bwd")
+    dev = _device()
+    ld = _row_view(s, rows, K, (s.dtype,), dev, "topk_kl_fwd_bwd.s")
+    ldv = _row_view(t_val, rows, k, tuple(_DT), dev, "topk_kl_fwd_bwd.t_val")
+    ldi = _row_view(t_idx, rows, k, _INDEX, dev, "topk_kl_fwd_bwd.t_idx")
+    ldd, p_d, dd = 0, None, s.dtype
+    if dlogits is not None:
+        ldd = _row_view(dlogits, rows, K, _F32_BF16 if s.dtype is torch.float32 else (s.dtype,), dev, "topk_kl_fwd_bwd.dlogits")
+        p_d, dd = dlogits.data_ptr(), dlogits.dtype
+    one = (rows,)
+    p_r, p_l = _flat(loss_rows, one, _F32, dev, "topk_kl_fwd_bwd.loss_rows"), _flat(loss, (1,), _F32, dev, "topk_kl_fwd_bwd.loss")
+    p_t, p_w = _flat(t_lse, one, _F32, dev, "topk_kl_fwd_bwd.t_lse"), _flat(row_weight, one, _F32, dev, "topk_kl_fwd_bwd.row_weight")
+    check(_lib.load().lt_topk_kl_fwd_bwd(s.data_ptr(), _DT[s.dtype], ld, t_val.data_ptr(), _DT[t_val.dtype], ldv, t_idx.data_ptr(), t_idx.dtype is torch.int64, ldi, p_t, p_w,
+                                         inv_temp, coef, p_r, p_l, p_d, _DT[dd], ldd, rows, K, k, _raw_stream(dev) if _raw_stream is not None else _stream()),
+          "lt_topk_kl_fwd_bwd")
 
 
 def symmetrize_bf16(d: Tensor, g: Tensor, batch: int, n: int, ld: int) -> None:
@@ -563,6 +594,10 @@ def rope_apply(qkv: Tensor, sin_t: Tensor, cos_t: Tensor, B: int, N: int, H: int
     check(_lib.load().lt_rope_apply(_p(qkv), _p(sin_t), _p(cos_t), B, N, H, dh, prefix, int(inverse), _stream()), "lt_rope_apply")
 
 
+_ROPE = struct.Struct("@7P12q12i")          # lt_rope_axes_desc (_lib.RopeAxesDesc)
+_POS = (torch.int32, torch.float32)
+
+
 def rope_axes(x: Tensor, out: Tensor, pos: Tensor, freqs: Tensor, axis: Tensor, prefix: int = 0, interleaved: bool = False, inverse: bool = False,
               x2: Optional[Tensor] = None, out2: Optional[Tensor] = None) -> None:
     """Rotary positions with several axes: pair i of every head of x [B, N, H, dh] (bf16, f16 or f32, strided views allowed) turns by
@@ -570,38 +605,35 @@ def rope_axes(x: Tensor, out: Tensor, pos: Tensor, freqs: Tensor, axis: Tensor, 
     [N - prefix, axes] or, per sample, [B, N - prefix, axes], 1 to 4 axes; freqs f32 and axis int32 [dh / 2] (`rope_axes_tables`); tokens < prefix and pairs of an
     axis outside the table pass through.  inverse: the transposed rotation, i.e. the gradient (lt_rope_axes)."""
     who = "rope_axes"
-    if x.dim() != 4 or x.dtype not in _DT:
-        raise ValueError(f"{who}.x: expected a [batch, token, head, d] view of bfloat16, float16 or float32, got {x.dtype} of shape {tuple(x.shape)}")
-    B, N, H, dh = x.shape
+    dt = x.dtype
+    if x.dim() != 4 or dt not in _DT:
+        raise ValueError(f"{who}.x: expected a [batch, token, head, d] view of bfloat16, float16 or float32, got {dt} of shape {tuple(x.shape)}")
+    sx = x.shape
+    B, N, H, dh = sx
     if dh % 8 or not 8 <= dh <= 256:
         raise ValueError(f"{who}: head_dim must be a multiple of 8 from 8 to 256, got {dh}")
     if not 0 <= prefix <= N:
         raise ValueError(f"{who}: prefix must lie between 0 and the {N} tokens, got {prefix}")
     if (x2 is None) != (out2 is None):
         raise ValueError(f"{who}: x2 and out2 come together")
-    dt, n = x.dtype, N - prefix
-    _strided(x, (B, N, H, dh), dt, who + ".x")
-    _strided(out, (B, N, H, dh), dt, who + ".out", True)
     if pos.dim() not in (2, 3) or not 1 <= pos.shape[-1] <= 4:
         raise ValueError(f"{who}.pos: expected [tokens, axes] or [batch, tokens, axes] with 1 to 4 axes, got {tuple(pos.shape)}")
-    A = pos.shape[-1]
-    _flat(pos, (n, A) if pos.dim() == 2 else (B, n, A), (torch.int32, torch.float32), who + ".pos")
-    _flat(freqs, (dh // 2,), (torch.float32,), who + ".freqs")
-    _flat(axis, (dh // 2,), (torch.int32,), who + ".axis")
-    d = RopeAxesDesc()
-    d.B, d.N, d.H, d.dh, d.dtype, d.prefix, d.axes = B, N, H, dh, _DT[dt], prefix, A
-    d.pos_per_batch, d.pos_float, d.interleaved, d.inverse = int(pos.dim() == 3), int(pos.dtype == torch.float32), int(interleaved), int(inverse)
-    d.x, d.out, d.pos, d.freqs, d.axis = _p(x), _p(out), _p(pos), _p(freqs), _p(axis)
-    d.sx[:], d.so[:] = x.stride()[:3], out.stride()[:3]
-    if x2 is not None:
-        if x2.dim() != 4:
+    dev, n, A, own = _device(), N - prefix, pos.shape[-1], pos.dim() == 3
+    ts = _strided(x, sx, dt, dev, who + ".x") + _strided(out, sx, dt, dev, who + ".out", True)
+    p_pos = _flat(pos, (B, n, A) if own else (n, A), _POS, dev, who + ".pos")
+    p_f, p_a = _flat(freqs, (dh // 2,), _F32, dev, who + ".freqs"), _flat(axis, (dh // 2,), _KEY_LENS, dev, who + ".axis")
+    H2 = p_x2 = p_o2 = 0
+    if x2 is None:
+        ts += _NO_STRIDE * 2
+    else:
+        if x2.dim() != 4 or x2.shape[2] < 1:
             raise ValueError(f"{who}.x2: expected a [batch, token, head, d] view, got shape {tuple(x2.shape)}")
-        d.H2 = x2.shape[2]
-        _strided(x2, (B, N, d.H2, dh), dt, who + ".x2")
-        _strided(out2, (B, N, d.H2, dh), dt, who + ".out2", True)
-        d.x2, d.out2 = _p(x2), _p(out2)
-        d.sx2[:], d.so2[:] = x2.stride()[:3], out2.stride()[:3]
-    check(_lib.load().lt_rope_axes(C.byref(d), _stream()), "lt_rope_axes")
+        H2 = x2.shape[2]
+        ts += _strided(x2, (B, N, H2, dh), dt, dev, who + ".x2") + _strided(out2, (B, N, H2, dh), dt, dev, who + ".out2", True)
+        p_x2, p_o2 = x2.data_ptr(), out2.data_ptr()
+    d = _ROPE.pack(x.data_ptr(), p_x2, out.data_ptr(), p_o2, p_pos, p_f, p_a, *ts, B, N, H, H2, dh, _DT[dt], prefix, A, own, pos.dtype is torch.float32,
+                   bool(interleaved), bool(inverse))
+    check(_lib.load().lt_rope_axes(d, _raw_stream(dev) if _raw_stream is not None else _stream()), "lt_rope_axes")
 
 
 def rope_axes_tables(dh: int, pairs: Any, base: float = 10000.0, shared_spectrum: bool = False, device: Any = None) -> Any:
@@ -685,50 +717,64 @@ def attention_bwd(qkv: Tensor, out: Tensor, dout: Tensor, lse: Tensor, ws: Tenso
           "lt_attention_bwd")
 
 
+@functools.lru_cache(maxsize=4096)
 def cross_attention_fwd_ws_floats(B: int, Nq: int, Nk: int, H: int, Hkv: int, dh: int) -> int:
     return int(_lib.load().lt_cross_attention_fwd_ws_floats(B, Nq, Nk, H, Hkv, dh))
 
 
+@functools.lru_cache(maxsize=4096)
 def cross_attention_bwd_ws_floats(B: int, Nq: int, Nk: int, H: int, Hkv: int, dh: int) -> int:
     return int(_lib.load().lt_cross_attention_bwd_ws_floats(B, Nq, Nk, H, Hkv, dh))
 
 
-def _xattn_desc(who: str, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optional[Tensor], scale: float, key_lens: Optional[Tensor],
-                key_mask: Optional[Tensor], ws: Optional[Tensor], ws_floats: Any, written: bool) -> CrossAttentionDesc:
+_XATTN = struct.Struct("@11P24q7ifPq")      # lt_cross_attention_desc (_lib.CrossAttentionDesc)
+_KEY_MASK, _KEY_LENS = (torch.bool, torch.uint8), (torch.int32,)
+
+
+def _xattn(who: str, fn: str, ws_floats: Any, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optional[Tensor], scale: float, key_lens: Optional[Tensor],
+           key_mask: Optional[Tensor], ws: Optional[Tensor], grads: Any = None) -> None:
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"{who}: q, k, v are [batch, token, head, d] views, got {tuple(q.shape)} and {tuple(k.shape)}")
-    B, Nq, H, dh = q.shape
-    Nk, Hkv = k.shape[1], k.shape[2]
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{who}: q must be bfloat16 or float16, got {q.dtype}")
+    sq = q.shape
+    B, Nq, H, dh = sq
+    _, Nk, Hkv, _ = k.shape
+    dt = q.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise ValueError(f"{who}: q must be bfloat16 or float16, got {dt}")
     if Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError(f"{who}: the query heads ({H}) must be a multiple of the key heads ({Hkv})")
     if dh % 8 or not 8 <= dh <= 128:
         raise ValueError(f"{who}: head_dim must be a multiple of 8 from 8 to 128, got {dh}")
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"{who}: scale must be positive and finite, got {scale}")
-    dt = q.dtype
-    _strided(q, (B, Nq, H, dh), dt, who + ".q")
-    _strided(k, (B, Nk, Hkv, dh), dt, who + ".k")
-    _strided(v, (B, Nk, Hkv, dh), dt, who + ".v")
-    _strided(out, (B, Nq, H, dh), dt, who + ".out", written)
-    _flat(lse, (B, H, Nq), (torch.float32,), who + ".lse")
-    _flat(key_lens, (B,), (torch.int32,), who + ".key_lens")
-    _flat(key_mask, (B, Nk), (torch.bool, torch.uint8), who + ".key_mask")
-    need = ws_floats(B, Nq, Nk, H, Hkv, dh)
-    if ws is None:
-        ws = torch.empty(need, device=q.device, dtype=torch.float32) if need else None
-    elif ws.dtype != torch.float32 or not ws.is_contiguous() or ws.numel() < need:
-        raise ValueError(f"{who}.ws: expected at least {need} contiguous float32, got {ws.numel()} of {ws.dtype}")
+    dev = _device()
+    sk = (B, Nk, Hkv, dh)
+    tq, tk, tv = _strided(q, sq, dt, dev, who + ".q"), _strided(k, sk, dt, dev, who + ".k"), _strided(v, sk, dt, dev, who + ".v")
+    to = _strided(out, sq, dt, dev, who + ".out", grads is None)
+    p_lse = _flat(lse, (B, H, Nq), _F32, dev, who + ".lse")
+    p_len, p_mask = _flat(key_lens, (B,), _KEY_LENS, dev, who + ".key_lens"), _flat(key_mask, (B, Nk), _KEY_MASK, dev, who + ".key_mask")
+    if grads is None:
+        p_g, t_g = (0, 0, 0, 0), _NO_STRIDE * 4
     else:
-        _here(ws, who + ".ws")
-    d = CrossAttentionDesc()
-    d.B, d.Nq, d.Nk, d.H, d.Hkv, d.dh, d.dtype, d.scale = B, Nq, Nk, H, Hkv, dh, _DT[dt], scale
-    d.q, d.k, d.v, d.out, d.lse, d.key_lens, d.key_mask = _p(q), _p(k), _p(v), _p(out), _p(lse), _p(key_lens), _p(key_mask)
-    d.sq[:], d.sk[:], d.sv[:], d.so[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3], out.stride()[:3]
-    d.ws, d.ws_floats = _p(ws), (ws.numel() if ws is not None else 0)
-    d._keep = ws      # (a workspace made here lives as long as the descriptor, i.e. as a recorded launch)
-    return d
+        do, dq, dk, dv = grads
+        t_g = (_strided(do, sq, dt, dev, who + ".dout") + _strided(dq, sq, dt, dev, who + ".dq", True) + _strided(dk, sk, dt, dev, who + ".dk", True)
+               + _strided(dv, sk, dt, dev, who + ".dv", True))
+        p_g = (do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    need = ws_floats(B, Nq, Nk, H, Hkv, dh)
+    made = None
+    if ws is None:
+        if need:
+            ws = made = torch.empty(need, device=q.device, dtype=torch.float32)
+    elif ws.dtype is not torch.float32 or not ws.is_contiguous() or ws.numel() < need or (need and ws.data_ptr() & 15):
+        raise ValueError(f"{who}.ws: expected at least {need} contiguous, 16-byte aligned float32, got {ws.numel()} of {ws.dtype}")
+    elif ws.get_device() != dev:
+        raise _elsewhere(ws, dev, who + ".ws")
+    d = _XATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p_lse, p_len, p_mask, *p_g, *tq, *tk, *tv, *to, *t_g,
+                    B, Nq, Nk, H, Hkv, dh, _DT[dt], scale, *((ws.data_ptr(), ws.numel()) if need else (0, 0)))
+    if made is not None:
+        d = _Desc(d)
+        d.keep = made
+    check(getattr(_lib.load(), fn)(d, _raw_stream(dev) if _raw_stream is not None else _stream()), fn)
 
 
 def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optional[Tensor], scale: float, key_lens: Optional[Tensor] = None,
@@ -737,8 +783,7 @@ def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optio
     allowed, H a multiple of Hkv); lse f32 [B, H, Nq] (needed by the backward) or None.  key_lens int32 [B], key_mask bool / uint8 [B, Nk]: which keys
     are visible; a row without one gives out = 0, lse = -inf.  ws: f32 scratch of `cross_attention_fwd_ws_floats` elements, allocated
     here when None; calls that may run at the same time need their own (lt_cross_attention_fwd)."""
-    d = _xattn_desc("cross_attention_fwd", q, k, v, out, lse, scale, key_lens, key_mask, ws, cross_attention_fwd_ws_floats, True)
-    check(_lib.load().lt_cross_attention_fwd(C.byref(d), _stream()), "lt_cross_attention_fwd")
+    _xattn("cross_attention_fwd", "lt_cross_attention_fwd", cross_attention_fwd_ws_floats, q, k, v, out, lse, scale, key_lens, key_mask, ws)
 
 
 def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tensor, lse: Tensor, dq: Tensor, dk: Tensor, dv: Tensor, scale: float,
@@ -746,18 +791,9 @@ def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, dout: Tens
     """dq, dk, dv (overwritten; strided views allowed) of `cross_attention_fwd` from its out and lse and the upstream gradient dout.  Gradients of
     broadcast inputs (stride 0) come back per batch entry, those of shared key heads summed over the heads that read them; keys that are
     not visible get zeros.  ws: f32 scratch of `cross_attention_bwd_ws_floats` elements (lt_cross_attention_bwd)."""
-    who = "cross_attention_bwd"
     if lse is None:
-        raise ValueError(f"{who}.lse: the forward's lse is needed")
-    d = _xattn_desc(who, q, k, v, out, lse, scale, key_lens, key_mask, ws, cross_attention_bwd_ws_floats, False)
-    dt, sq, sk = q.dtype, tuple(q.shape), tuple(k.shape)
-    _strided(dout, sq, dt, who + ".dout")
-    _strided(dq, sq, dt, who + ".dq", True)
-    _strided(dk, sk, dt, who + ".dk", True)
-    _strided(dv, sk, dt, who + ".dv", True)
-    d.dout, d.dq, d.dk, d.dv = _p(dout), _p(dq), _p(dk), _p(dv)
-    d.sdo[:], d.sdq[:], d.sdk[:], d.sdv[:] = dout.stride()[:3], dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
-    check(_lib.load().lt_cross_attention_bwd(C.byref(d), _stream()), "lt_cross_attention_bwd")
+        raise ValueError("cross_attention_bwd.lse: the forward's lse is needed")
+    _xattn("cross_attention_bwd", "lt_cross_attention_bwd", cross_attention_bwd_ws_floats, q, k, v, out, lse, scale, key_lens, key_mask, ws, (dout, dq, dk, dv))
 
 
 # ------------------------------------------------------------------------------------------ head pieces

@@ -90,3 +90,16 @@ def test_topk_c_entry_refuses(at, v):
 
 def test_topk_without_rows_is_no_error():
     assert _lib.load().lt_topk_kl_fwd_bwd(None, 0, 50, None, 2, 4, None, 1, 4, None, None, 1.0, 1.0, None, None, None, 0, 50, 0, 50, 4, None) == 0
+
+
+def test_packed_descriptors_match_the_structures():
+    """The front ends hand over packed bytes: same size and order as the declared structures."""
+    for packer, cls, n in ((ops._ROPE, _lib.RopeAxesDesc, 31), (ops._XATTN, _lib.CrossAttentionDesc, 45)):
+        assert packer.size == C.sizeof(cls)
+        vals = list(range(1, n + 1))
+        d = cls.from_buffer_copy(packer.pack(*vals))
+        got = []
+        for name, _ in cls._fields_:
+            v = getattr(d, name)
+            got += list(v) if hasattr(v, "__len__") else [v]
+        assert got == vals
