@@ -209,7 +209,7 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
 
 // Tiled forward: a workgroup owns 4 waves x QT x 32 query rows of one (batch entry, key head) and walks its share of the keys in chunks of 64.
 template <bool F16, int HD, int QT>
-__global__ __launch_bounds__(NT) void xattn_fwd_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (row_img<HD>() + tr_img<HD>() + KC * 4)];
   constexpr int BUF = row_img<HD>() + tr_img<HD>() + KC * 4;
   int bh, item;
@@ -336,7 +336,7 @@ template <int HD> struct KeyTile {
 };
 
 template <bool F16, int HD>
-__global__ __launch_bounds__(NT) void xattn_fwd_few_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(const XArgs a) {
   constexpr int OST = HD * 32 + 4;   // floats between the rows of a wave's partial output
   __shared__ __attribute__((aligned(16))) char smem[4 * 32 * OST * 4 + 4 * 32 * 8];
   int bh, split;
@@ -462,7 +462,7 @@ __device__ __forceinline__ float row_start(float lse, float scale) { return lse 
 
 // dQ: a workgroup owns 128 query rows and walks its share of the keys; D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
 template <bool F16, int HD>
-__global__ __launch_bounds__(NT) void xattn_dq_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
   constexpr int BUF = 2 * row_img<HD>() + tr_img<HD>() + KC * 4;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   int bh, item;
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(NT) void xattn_dq_kernel(const XArgs a) {
 
 // dK / dV: a wave owns 32 keys (K, V fragments and both accumulators in registers), the query rows pass through LDS in chunks of 64.
 template <bool F16, int HD>
-__global__ __launch_bounds__(NT) void xattn_dkdv_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const XArgs a) {
   constexpr int BUF = 2 * row_img<HD>() + 2 * tr_img<HD>() + 2 * KC * 4;
   __shared__ __attribute__((aligned(16))) char smem[BUF];
   int bh, item;
@@ -665,7 +665,7 @@ __global__ __launch_bounds__(NT) void xattn_dkdv_kernel(const XArgs a) {
 // over K / V.  Each wave owns key tiles; S is formed in both orientations (lane -> key for dK / dV, lane -> query for dQ): the second set of
 // products costs less than turning dS through LDS, and the pass is bound by memory.
 template <bool F16, int HD>
-__global__ __launch_bounds__(NT) void xattn_bwd_few_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(const XArgs a) {
   constexpr int IMG = 32 * HD * 64, OST = HD * 32 + 4;
   constexpr int TAIL = 4 * 32 * OST * 4, HEAD = 6 * IMG + 2 * 32 * 4;
   __shared__ __attribute__((aligned(16))) char smem[TAIL > HEAD ? TAIL : HEAD];
