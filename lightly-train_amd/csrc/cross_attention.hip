@@ -99,16 +99,17 @@ template <int HD> __device__ __forceinline__ s16x8 tr_frag(const char* img, int 
   const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(img + ((q + 2) * 2 * HD + b) * 128 + inner));
   return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// KC tokens between memory and the images, through registers (the next chunk's loads stay in flight while a chunk is computed)
+// KC tokens between memory and the images, through registers (the next chunk's loads stay in flight while a chunk is computed).  Hidden keys are
+// loaded like the others -- a load that waited for its mask byte would expose two latencies per chunk -- and become zeros on the way to LDS.
 template <int HD> struct Chunk {
   static constexpr int CPR = 4 * HD, PER = KC * CPR / NT;
   uint4 u[PER];
-  __device__ __forceinline__ void load_keys(const uint16_t* base, int64_t sn, int tok0, int end, const uint8_t* mask, int dh) {
+  __device__ __forceinline__ void load_keys(const uint16_t* base, int64_t sn, int tok0, int end, int dh) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR, tok = tok0 + r;
+      const int idx = threadIdx.x + NT * i, c = idx % CPR, tok = tok0 + idx / CPR;
       u[i] = make_uint4(0, 0, 0, 0);
-      if (tok < end && c * 8 < dh && (!mask || mask[tok])) u[i] = *reinterpret_cast<const uint4*>(base + tok * sn + c * 8);
+      if (tok < end && c * 8 < dh) u[i] = *reinterpret_cast<const uint4*>(base + tok * sn + c * 8);
     }
   }
   __device__ __forceinline__ void load_rows(const uint16_t* base, const Strides& s, int r0, int R, int Nq, int dh) {
@@ -121,6 +122,11 @@ template <int HD> struct Chunk {
         u[i] = *reinterpret_cast<const uint4*>(base + n * s.n + g * s.h + c * 8);
       }
     }
+  }
+  __device__ __forceinline__ void hide(const uint8_t (&m)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (!m[i]) u[i] = make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ void store_rows(char* img) const {
 #pragma unroll
@@ -135,6 +141,31 @@ template <int HD> struct Chunk {
       const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR;
       *reinterpret_cast<uint4*>(img + tr_off<HD>(r, c)) = u[i];
     }
+  }
+};
+// K and V of a chunk with the mask bytes of the rows that this thread carries, and the score start value (0 / -inf) of key threadIdx.x
+template <int HD> struct KeyChunk {
+  Chunk<HD> k, v;
+  uint8_t m[Chunk<HD>::PER], mb;
+  bool in;
+  __device__ __forceinline__ void load(const XArgs& a, const uint16_t* kb, const uint16_t* vb, const uint8_t* mask, int c, int kend) {
+    k.load_keys(kb, a.sk.n, c * KC, kend, a.dh);
+    v.load_keys(vb, a.sv.n, c * KC, kend, a.dh);
+    in = c * KC + (int)threadIdx.x < kend;
+    if (mask) {
+#pragma unroll
+      for (int i = 0; i < Chunk<HD>::PER; ++i) {
+        const int tok = c * KC + (threadIdx.x + NT * i) / Chunk<HD>::CPR;
+        m[i] = tok < kend ? mask[tok] : 0;
+      }
+      mb = threadIdx.x < KC && in ? mask[c * KC + threadIdx.x] : 0;
+    }
+  }
+  __device__ __forceinline__ float hide(const uint8_t* mask) {   // returns the start value
+    if (!mask) return in ? 0.f : -INFINITY;
+    k.hide(m);
+    v.hide(m);
+    return mb ? 0.f : -INFINITY;
   }
 };
 template <int HD> constexpr int row_img() { return KC * row_stride<HD>(); }
@@ -222,16 +253,12 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
   const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
   const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
 
-  Chunk<HD> kr, vr;
-  float bias = 0.f;
-  auto load = [&](int c) {
-    kr.load_keys(kb, a.sk.n, c * KC, kend, mask, a.dh);
-    vr.load_keys(vb, a.sv.n, c * KC, kend, mask, a.dh);
-    if (threadIdx.x < KC) { const int key = c * KC + threadIdx.x; bias = key < kend && (!mask || mask[key]) ? 0.f : -INFINITY; }
-  };
+  KeyChunk<HD> in;
+  auto load = [&](int c) { in.load(a, kb, vb, mask, c, kend); };
   auto store = [&](int buf) {
-    kr.store_rows(smem + buf * BUF);
-    vr.store_tr(smem + buf * BUF + row_img<HD>());
+    const float bias = in.hide(mask);
+    in.k.store_rows(smem + buf * BUF);
+    in.v.store_tr(smem + buf * BUF + row_img<HD>());
     if (threadIdx.x < KC) *reinterpret_cast<float*>(smem + buf * BUF + row_img<HD>() + tr_img<HD>() + threadIdx.x * 4) = bias;
   };
   if (c_lo < c_hi) load(c_lo);
@@ -328,6 +355,11 @@ template <int HD> struct KeyTile {
 #pragma unroll
     for (int ks = 0; ks < 2 * HD; ++ks) f[ks] = ld8(base + key * sn + ks * 16 + hi * 8, ok && ks * 16 + hi * 8 < dh);
   }
+  __device__ __forceinline__ void hide(bool ok) {
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks)
+      if (!ok) f[ks] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
   __device__ __forceinline__ void store_tr(char* img) const {   // token l % 32, chunk 2 ks + hi
     const int l = lane();
 #pragma unroll
@@ -351,12 +383,14 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
   char* img = smem + wave * (32 * HD * 64);
 
   KeyTile<HD> kf, vf;
-  bool ok = false;
+  bool in = false;
+  uint8_t mb = 1;
   auto load = [&](int t) {
     const int key = t * 32 + (l & 31);
-    ok = t < t_hi && key < kend && (!mask || mask[key]);
-    kf.load(kb, a.sk.n, key, ok, a.dh);
-    vf.load(vb, a.sv.n, key, ok, a.dh);
+    in = t < t_hi && key < kend;
+    kf.load(kb, a.sk.n, key, in, a.dh);
+    vf.load(vb, a.sv.n, key, in, a.dh);
+    if (mask) mb = in ? mask[key] : 0;
   };
   load(t_lo + wave);
   const int r = l & 31, g = r / a.Nq, n = r - g * a.Nq;
@@ -370,9 +404,12 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
   float m = M_NONE, lsum = 0.f;
   const float c = a.scale * LOG2E;
   for (int t = t_lo + wave; t < t_hi; t += 4) {
+    const bool ok = in && mb;
     const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
     f32x16 s[1] = {splat(0.f)};
     if (seen != 0xffffffffu) {
+      kf.hide(ok);
+      vf.hide(ok);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[0][e] = (seen >> crow(e, hi)) & 1 ? 0.f : -INFINITY;
     }
@@ -474,18 +511,14 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
   const uint16_t* kb = a.k + b * a.sk.b + hk * a.sk.h;
   const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
   const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
-  Chunk<HD> kr, vr;
-  float bias = 0.f;
-  auto load = [&](int c) {
-    kr.load_keys(kb, a.sk.n, c * KC, kend, mask, a.dh);
-    vr.load_keys(vb, a.sv.n, c * KC, kend, mask, a.dh);
-    if (threadIdx.x < KC) { const int key = c * KC + threadIdx.x; bias = key < kend && (!mask || mask[key]) ? 0.f : -INFINITY; }
-  };
+  KeyChunk<HD> in;
+  auto load = [&](int c) { in.load(a, kb, vb, mask, c, kend); };
   auto store = [&](int buf) {
     char* p = smem + buf * BUF;
-    kr.store_rows(p);
-    vr.store_rows(p + row_img<HD>());
-    kr.store_tr(p + 2 * row_img<HD>());
+    const float bias = in.hide(mask);
+    in.k.store_rows(p);
+    in.v.store_rows(p + row_img<HD>());
+    in.k.store_tr(p + 2 * row_img<HD>());
     if (threadIdx.x < KC) *reinterpret_cast<float*>(p + 2 * row_img<HD>() + tr_img<HD>() + threadIdx.x * 4) = bias;
   };
   if (c_lo < c_hi) load(c_lo);
@@ -683,12 +716,14 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
   char* Kt = smem + (2 + wave) * IMG;
   float* st = reinterpret_cast<float*>(smem + 6 * IMG);
   KeyTile<HD> kn, vn;
-  bool okn = false;
+  bool in = false;
+  uint8_t mb = 1;
   auto load = [&](int t) {
     const int key = t * 32 + (l & 31);
-    okn = t < t_hi && key < kend && (!mask || mask[key]);
-    kn.load(kb, a.sk.n, key, okn, a.dh);
-    vn.load(vb, a.sv.n, key, okn, a.dh);
+    in = t < t_hi && key < kend;
+    kn.load(kb, a.sk.n, key, in, a.dh);
+    vn.load(vb, a.sv.n, key, in, a.dh);
+    if (mask) mb = in ? mask[key] : 0;
   };
   load(t_lo + wave);
   const int r = l & 31, g = r / a.Nq, n = r - g * a.Nq;
@@ -719,9 +754,13 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
   for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
   __syncthreads();
   for (int t = t_lo + wave; t < t_hi; t += 4) {
-    const KeyTile<HD> kf = kn, vf = vn;
-    const bool seen = okn;
+    KeyTile<HD> kf = kn, vf = vn;
+    const bool seen = in && mb;
     const uint32_t all = (uint32_t)__builtin_amdgcn_ballot_w64(seen);
+    if (all != 0xffffffffu) {
+      kf.hide(seen);
+      vf.hide(seen);
+    }
     load(t + 4);
     kf.store_tr(Kt);
     f32x16 dk[HD], dv[HD];
@@ -832,47 +871,59 @@ struct Plan { bool few; int tiles, splits; };
 
 int round_up8(int64_t x) { return (int)((x + 7) / 8 * 8); }
 
-// `blocks` workgroups without a split along an axis of `chunks` pieces: split until the card has about `want` workgroups, with at least `least`
-// pieces left to each
-int split_for(int64_t blocks, int chunks, int want, int least) {
-  if (blocks <= 0 || blocks >= want || chunks < 2 * least) return 1;
-  int64_t s = (want + blocks - 1) / blocks;
-  if (s > chunks / least) s = chunks / least;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : (int)s;
+// Into how many pieces the contracted axis (`chunks` steps) of `blocks` workgroups is cut, so that the last round of workgroups over the card's
+// `slots` does not run half empty: the smallest estimated time of rounds * (steps + 2) * us_step, plus joining the fp32 partials (`mbytes` per
+// piece, written and read at ~4.5 TB/s, and a launch).  Estimates only rank the cuts; every cut gives a right result.
+int split_for(int64_t blocks, int chunks, int slots, double us_step, double mbytes) {
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && s <= (chunks > 1 ? chunks / 2 : 1); ++s) {
+    const double rounds = (double)((blocks * s + slots - 1) / slots), steps = (double)((chunks + s - 1) / s) + 2;
+    const double t = rounds * steps * us_step + (s > 1 ? 4. + 2. * s * mbytes / 4.5 : 0.);
+    if (t < least) { least = t; best = s; }
+  }
+  return best;
 }
 bool few_rows(int R) { return R <= 32; }
-int row_tiles(int HD) { return HD <= 2 ? 2 : 1; }   // 32-row tiles per wave of the tiled forward
+// 32-row tiles per wave of the tiled forward: two share every K / V fragment read from LDS, where the registers hold them (head_dim <= 64) and 256-row
+// workgroups pad no more rows than 128-row ones
+int row_tiles(int HD, int R) { return HD <= 2 && lt_cdiv(R, 256) * 2 == lt_cdiv(R, 128) ? 2 : 1; }
 
+constexpr int SLOTS = 2 * CUS;     // workgroups of the tiled kernels that the card holds at a time
+// (us_step: a 64-token chunk of the tiled kernels at ~1 TFLOP/s a workgroup; a step of 4 x 32 keys of the few-row kernels)
 Plan fwd_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int64_t bh = (int64_t)B * Hkv;
-  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 32), 3 * CUS, 8)};
-  const int tiles = lt_cdiv(R, 128 * row_tiles(lt_cdiv(dh, 32)));
-  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), 2 * CUS, 4)};
+  const int HD = lt_cdiv(dh, 32);
+  const double mb = 4e-6 * bh * R * dh;
+  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 128), 3 * CUS, 1.5, mb)};
+  const int rows = 128 * row_tiles(HD, R), tiles = lt_cdiv(R, rows);
+  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), SLOTS, 4e-6 * rows * KC * HD * 32, mb)};
 }
-Plan dq_plan(int B, int R, int Nk, int Hkv) {
+Plan dq_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int64_t bh = (int64_t)B * Hkv;
-  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 32), 3 * CUS, 4)};
-  const int tiles = lt_cdiv(R, 128);
-  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), 2 * CUS, 4)};
+  const int HD = lt_cdiv(dh, 32), tiles = lt_cdiv(R, 128);
+  const double mb = 4e-6 * bh * R * dh;
+  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 128), SLOTS, 2.5, mb)};
+  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), SLOTS, 6e-6 * 128 * KC * HD * 32, mb)};
 }
-Plan dkdv_plan(int B, int R, int Nk, int Hkv) {
-  const int tiles = lt_cdiv(Nk, 128);
-  return {false, tiles, split_for((int64_t)B * Hkv * tiles, lt_cdiv(R, KC), 2 * CUS, 4)};
+Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
+  const int HD = lt_cdiv(dh, 32), tiles = lt_cdiv(Nk, 128);
+  const int64_t bh = (int64_t)B * Hkv;
+  return {false, tiles, split_for(bh * tiles, lt_cdiv(R, KC), SLOTS, 8e-6 * 128 * KC * HD * 32, 8e-6 * bh * Nk * dh)};
 }
 int64_t fwd_floats(int B, int R, int Nk, int Hkv, int dh) {
   const Plan p = fwd_plan(B, R, Nk, Hkv, dh);
   return p.splits > 1 ? (int64_t)p.splits * B * Hkv * R * (dh + 2) : 0;
 }
 int64_t dq_floats(int B, int R, int Nk, int Hkv, int dh) {
-  const Plan p = dq_plan(B, R, Nk, Hkv);
+  const Plan p = dq_plan(B, R, Nk, Hkv, dh);
   return p.splits > 1 ? (int64_t)p.splits * B * Hkv * R * dh : 0;
 }
 int64_t delta_floats(int B, int R, int Hkv) { return ((int64_t)B * Hkv * R + 3) / 4 * 4; }
 int64_t bwd_floats(int B, int R, int Nk, int Hkv, int dh) {
   int64_t n = dq_floats(B, R, Nk, Hkv, dh);
   if (few_rows(R)) return n;
-  const Plan p = dkdv_plan(B, R, Nk, Hkv);
+  const Plan p = dkdv_plan(B, R, Nk, Hkv, dh);
   const int64_t kv = p.splits > 1 ? 2 * (int64_t)p.splits * B * Hkv * Nk * dh : 0;
   return delta_floats(B, R, Hkv) + (n > kv ? n : kv);
 }
@@ -917,12 +968,13 @@ template <bool F16> void run_fwd(const XArgs& a, bool few, void* stream) {
   const int64_t items = (int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits;
   if (few) { XA_HD(xattn_fwd_few_kernel, (unsigned)items, F16) }
   else {
-    switch (lt_cdiv(a.dh, 32)) {
-      case 1: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 1, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
-      case 2: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 2, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
-      case 3: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 3, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
-      default: hipLaunchKernelGGL((xattn_fwd_kernel<F16, 4, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a); break;
-    }
+    const int HD = lt_cdiv(a.dh, 32), qt = row_tiles(HD, a.R);
+    if (HD == 1 && qt == 2) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 1, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
+    else if (HD == 2 && qt == 2) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 2, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
+    else if (HD == 1) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 1, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
+    else if (HD == 2) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 2, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
+    else if (HD == 3) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 3, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((xattn_fwd_kernel<F16, 4, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
   }
   if (a.splits > 1) {
     const int64_t n = (int64_t)a.B * a.Hkv * a.R * (a.dh / 4);
@@ -935,7 +987,7 @@ template <bool F16> void add_splits(const XArgs& a, const float* part, uint16_t*
 }
 template <bool F16> void run_bwd(XArgs a, float* ws, void* stream) {
   const int64_t bh8 = round_up8((int64_t)a.B * a.Hkv), rows = (int64_t)a.B * a.Hkv * a.R, keys = (int64_t)a.B * a.Hkv * a.Nk;
-  Plan p = dq_plan(a.B, a.R, a.Nk, a.Hkv);
+  Plan p = dq_plan(a.B, a.R, a.Nk, a.Hkv, a.dh);
   a.tiles = p.tiles; a.splits = p.splits;
   a.delta = ws;
   a.ws = p.few ? ws : ws + delta_floats(a.B, a.R, a.Hkv);
@@ -943,7 +995,7 @@ template <bool F16> void run_bwd(XArgs a, float* ws, void* stream) {
   else { XA_HD(xattn_dq_kernel, (unsigned)(bh8 * a.tiles * a.splits), F16) }
   if (a.splits > 1) add_splits<F16>(a, a.ws, a.dq, a.sdq, rows, a.R, a.Nq, a.G, stream);
   if (p.few || a.Nk == 0) return;
-  p = dkdv_plan(a.B, a.R, a.Nk, a.Hkv);
+  p = dkdv_plan(a.B, a.R, a.Nk, a.Hkv, a.dh);
   a.tiles = p.tiles; a.splits = p.splits;
   XA_HD(xattn_dkdv_kernel, (unsigned)(bh8 * a.tiles * a.splits), F16)
   if (a.splits > 1) {
@@ -1014,7 +1066,7 @@ extern "C" int lt_cross_attention_bwd(const lt_cross_attention_desc* d, void* st
   LT_CHECK_ARG(need == 0 || (d->ws && aligned16(d->ws) && d->ws_floats >= need), "lt_cross_attention_bwd: a workspace of %lld floats is needed (got %lld)", (long long)need,
                (long long)(d->ws ? d->ws_floats : 0));
   const int64_t bh8 = round_up8((int64_t)a.B * a.Hkv);
-  const Plan p1 = dq_plan(a.B, a.R, a.Nk, a.Hkv), p2 = dkdv_plan(a.B, a.R, a.Nk, a.Hkv);
+  const Plan p1 = dq_plan(a.B, a.R, a.Nk, a.Hkv, a.dh), p2 = dkdv_plan(a.B, a.R, a.Nk, a.Hkv, a.dh);
   LT_CHECK_ARG(bh8 * p1.tiles * p1.splits < (1ll << 31) && bh8 * p2.tiles * p2.splits < (1ll << 31), "lt_cross_attention_bwd: too many workgroups");
   if (d->dtype == LT_DT_F16) run_bwd<true>(a, d->ws, stream);
   else run_bwd<false>(a, d->ws, stream);
