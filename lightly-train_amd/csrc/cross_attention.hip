@@ -99,27 +99,51 @@ template <int HD> __device__ __forceinline__ s16x8 tr_frag(const char* img, int 
   const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(img + ((q + 2) * 2 * HD + b) * 128 + inner));
   return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// KC tokens between memory and the images, through registers (the next chunk's loads stay in flight while a chunk is computed).  Hidden keys are
-// loaded like the others -- a load that waited for its mask byte would expose two latencies per chunk -- and become zeros on the way to LDS.
+// KC tokens between memory and the images, through registers (the next chunk's loads stay in flight while a chunk is computed).  The loads go through
+// a buffer descriptor that begins at the chunk's first token: a thread's offsets are the same for every chunk, no address arithmetic is left to
+// the vector units (it was half of their instructions), and tokens past the end, or columns past head_dim, read as zeros.
+constexpr int64_t MAX_STEP = 1 << 24;   // elements between two tokens: 64 tokens stay inside 31 bits
+struct Window {
+  __amdgpu_buffer_rsrc_t r;
+  // `tokens` rows from `base`, sn elements apart, of which dh are read
+  __device__ __forceinline__ Window(const uint16_t* base, int64_t sn, int tokens, int dh) {
+    const uint32_t bytes = tokens > 0 ? (uint32_t)(((int64_t)min(tokens, KC) - 1) * sn + dh) * 2u : 0u;
+    const uint64_t p = (uint64_t)base;
+    const uint64_t q = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p) |
+                       ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32)) << 32);
+    r = __builtin_amdgcn_make_buffer_rsrc((void*)q, 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+  }
+  __device__ __forceinline__ uint4 load(uint32_t off) const { return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0)); }
+};
 template <int HD> struct Chunk {
   static constexpr int CPR = 4 * HD, PER = KC * CPR / NT;
   uint4 u[PER];
-  __device__ __forceinline__ void load_keys(const uint16_t* base, int64_t sn, int tok0, int end, int dh) {
+  uint32_t off[PER];
+  __device__ __forceinline__ void offsets(int64_t sn, int dh) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + NT * i, c = idx % CPR, tok = tok0 + idx / CPR;
-      u[i] = make_uint4(0, 0, 0, 0);
-      if (tok < end && c * 8 < dh) u[i] = *reinterpret_cast<const uint4*>(base + tok * sn + c * 8);
+      const int idx = threadIdx.x + NT * i, c = idx % CPR;
+      off[i] = c * 8 < dh ? (uint32_t)(idx / CPR) * (uint32_t)sn * 2u + c * 16u : 0xfffffff0u;
     }
   }
-  __device__ __forceinline__ void load_rows(const uint16_t* base, const Strides& s, int r0, int R, int Nq, int dh) {
+  __device__ __forceinline__ void load(const uint16_t* base, int64_t sn, int tok0, int end, int dh) {
+    const Window w(base + (int64_t)tok0 * sn, sn, end - tok0, dh);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + NT * i, r = r0 + idx / CPR, c = idx % CPR;
-      u[i] = make_uint4(0, 0, 0, 0);
-      if (r < R && c * 8 < dh) {
-        const int g = r / Nq, n = r - g * Nq;
-        u[i] = *reinterpret_cast<const uint4*>(base + n * s.n + g * s.h + c * 8);
+    for (int i = 0; i < PER; ++i) u[i] = w.load(off[i]);
+  }
+  // query rows r0 .. r0 + KC - 1; n0, g0: token and head of row r0
+  __device__ __forceinline__ void load_rows(const uint16_t* base, const Strides& s, int r0, int g0, int n0, int R, int Nq, int dh) {
+    if (n0 + KC <= Nq || r0 - n0 + Nq >= R) {   // the chunk lies in one head, or in the last
+      load(base + (int64_t)g0 * s.h, s.n, n0, Nq, dh);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int idx = threadIdx.x + NT * i, r = r0 + idx / CPR, c = idx % CPR;
+        u[i] = make_uint4(0, 0, 0, 0);
+        if (r < R && c * 8 < dh) {
+          const int g = r / Nq, n = r - g * Nq;
+          u[i] = *reinterpret_cast<const uint4*>(base + n * s.n + g * s.h + c * 8);
+        }
       }
     }
   }
@@ -143,14 +167,19 @@ template <int HD> struct Chunk {
     }
   }
 };
-// K and V of a chunk with the mask bytes of the rows that this thread carries, and the score start value (0 / -inf) of key threadIdx.x
+// K and V of a chunk with the mask bytes of the rows that this thread carries, and the score start value (0 / -inf) of key threadIdx.x.  Hidden keys
+// are loaded like the others -- a load that waited for its mask byte would expose two latencies per chunk -- and become zeros on the way to LDS.
 template <int HD> struct KeyChunk {
   Chunk<HD> k, v;
   uint8_t m[Chunk<HD>::PER], mb;
   bool in;
+  __device__ __forceinline__ void offsets(const XArgs& a) {
+    k.offsets(a.sk.n, a.dh);
+    v.offsets(a.sv.n, a.dh);
+  }
   __device__ __forceinline__ void load(const XArgs& a, const uint16_t* kb, const uint16_t* vb, const uint8_t* mask, int c, int kend) {
-    k.load_keys(kb, a.sk.n, c * KC, kend, a.dh);
-    v.load_keys(vb, a.sv.n, c * KC, kend, a.dh);
+    k.load(kb, a.sk.n, c * KC, kend, a.dh);
+    v.load(vb, a.sv.n, c * KC, kend, a.dh);
     in = c * KC + (int)threadIdx.x < kend;
     if (mask) {
 #pragma unroll
@@ -178,7 +207,7 @@ __device__ __forceinline__ bool my_item(const XArgs& a, int per, int& bh, int& i
   item = i % per;
   return bh < a.B * a.Hkv;
 }
-__device__ __forceinline__ int key_end(const XArgs& a, int b) { return a.klen ? min(max(a.klen[b], 0), a.Nk) : a.Nk; }
+__device__ __forceinline__ int key_end(const XArgs& a, int b) { return __builtin_amdgcn_readfirstlane(a.klen ? min(max(a.klen[b], 0), a.Nk) : a.Nk); }
 
 // accumulators acc[HD] in C layout (lane -> row, registers -> d) to 16-bit rows / fp32 partial rows
 template <bool F16, int HD> __device__ __forceinline__ void put_row(uint16_t* dst, const f32x16 (&acc)[HD], float mul, int dh) {
@@ -254,6 +283,7 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
   const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
 
   KeyChunk<HD> in;
+  in.offsets(a);
   auto load = [&](int c) { in.load(a, kb, vb, mask, c, kend); };
   auto store = [&](int buf) {
     const float bias = in.hide(mask);
@@ -512,6 +542,7 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
   const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
   const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
   KeyChunk<HD> in;
+  in.offsets(a);
   auto load = [&](int c) { in.load(a, kb, vb, mask, c, kend); };
   auto store = [&](int buf) {
     char* p = smem + buf * BUF;
@@ -606,10 +637,14 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
   const uint16_t* qb = a.q + b * a.sq.b + (int64_t)hk * a.G * a.sq.h;
   const uint16_t* db_ = a.dout + b * a.sdo.b + (int64_t)hk * a.G * a.sdo.h;
   Chunk<HD> qr, dr;
+  qr.offsets(a.sq.n, a.dh);
+  dr.offsets(a.sdo.n, a.dh);
   float l_reg = 0.f, d_reg = 0.f;
+  int g0 = __builtin_amdgcn_readfirstlane(c_lo * KC / a.Nq), n0 = c_lo * KC - g0 * a.Nq;   // head and token of the next chunk's first row
   auto load = [&](int ch) {
-    qr.load_rows(qb, a.sq, ch * KC, a.R, a.Nq, a.dh);
-    dr.load_rows(db_, a.sdo, ch * KC, a.R, a.Nq, a.dh);
+    qr.load_rows(qb, a.sq, ch * KC, g0, n0, a.R, a.Nq, a.dh);
+    dr.load_rows(db_, a.sdo, ch * KC, g0, n0, a.R, a.Nq, a.dh);
+    for (n0 += KC; n0 >= a.Nq; n0 -= a.Nq) ++g0;
     if (threadIdx.x < KC) {
       const int r = ch * KC + threadIdx.x;
       l_reg = r < a.R ? row_start(a.lse[((int64_t)b * a.H + hk * a.G) * a.Nq + r], a.scale) : -INFINITY;   // rows of a group lie one after the other
@@ -654,9 +689,9 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
       for (int g = 0; g < 4; ++g) {
         const float4 x = *reinterpret_cast<const float4*>(st + t * 32 + 8 * g + 4 * hi);
         const float4 y = *reinterpret_cast<const float4*>(st + KC + t * 32 + 8 * g + 4 * hi);
-        s[4 * g] = seen ? x.x : -INFINITY; s[4 * g + 1] = seen ? x.y : -INFINITY; s[4 * g + 2] = seen ? x.z : -INFINITY; s[4 * g + 3] = seen ? x.w : -INFINITY;
+        s[4 * g] = x.x; s[4 * g + 1] = x.y; s[4 * g + 2] = x.z; s[4 * g + 3] = x.w;
         dp[4 * g] = y.x; dp[4 * g + 1] = y.y; dp[4 * g + 2] = y.z; dp[4 * g + 3] = y.w;
-      }
+      }   // (a hidden key's column is finite or, for rows without statistics, zero; its results are replaced by zeros at the end)
 #pragma unroll
       for (int ks = 0; ks < 2 * HD; ++ks) {
         s = mma<F16>(row_frag<HD>(Q, t, ks), kf.f[ks], s);
@@ -886,8 +921,8 @@ int split_for(int64_t blocks, int chunks, int slots, double us_step, double mbyt
 }
 bool few_rows(int R) { return R <= 32; }
 // 32-row tiles per wave of the tiled forward: two share every K / V fragment read from LDS, where the registers hold them (head_dim <= 64) and 256-row
-// workgroups pad no more rows than 128-row ones
-int row_tiles(int HD, int R) { return HD <= 2 && lt_cdiv(R, 256) * 2 == lt_cdiv(R, 128) ? 2 : 1; }
+// workgroups pad at most an eighth more rows than 128-row ones
+int row_tiles(int HD, int R) { return HD <= 2 && lt_cdiv(R, 256) * 16 <= lt_cdiv(R, 128) * 9 ? 2 : 1; }
 
 constexpr int SLOTS = 2 * CUS;     // workgroups of the tiled kernels that the card holds at a time
 // (us_step: a 64-token chunk of the tiled kernels at ~1 TFLOP/s a workgroup; a step of 4 x 32 keys of the few-row kernels)
@@ -929,9 +964,9 @@ int64_t bwd_floats(int B, int R, int Nk, int Hkv, int dh) {
 }
 
 bool strides_ok(const int64_t* s, int B, int N, int H) {
-  return (B == 1 || (s[0] >= 0 && s[0] % 8 == 0)) && (N == 1 || (s[1] >= 0 && s[1] % 8 == 0)) && (H == 1 || (s[2] >= 0 && s[2] % 8 == 0));
+  return (B == 1 || (s[0] >= 0 && s[0] % 8 == 0)) && (N == 1 || (s[1] >= 0 && s[1] % 8 == 0 && s[1] < MAX_STEP)) && (H == 1 || (s[2] >= 0 && s[2] % 8 == 0));
 }
-Strides st3(const int64_t* s) { return {s[0], s[1], s[2]}; }
+Strides st3(const int64_t* s, int N) { return {s[0], N == 1 ? 128 : s[1], s[2]}; }   // (a single token has no step: any will do)
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
@@ -951,7 +986,7 @@ int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
   a.q = (const uint16_t*)d->q; a.k = (const uint16_t*)d->k; a.v = (const uint16_t*)d->v;
   a.o = (const uint16_t*)d->out; a.out = (uint16_t*)d->out; a.lse = d->lse;
   a.klen = d->key_lens; a.kmask = d->key_mask;
-  a.sq = st3(d->sq); a.sk = st3(d->sk); a.sv = st3(d->sv); a.so = st3(d->so);
+  a.sq = st3(d->sq, d->Nq); a.sk = st3(d->sk, d->Nk); a.sv = st3(d->sv, d->Nk); a.so = st3(d->so, d->Nq);
   a.B = d->B; a.Nq = d->Nq; a.Nk = d->Nk; a.H = d->H; a.Hkv = d->Hkv; a.G = G; a.R = G * d->Nq; a.dh = d->dh; a.scale = d->scale;
   return LT_OK;
 }
@@ -1053,7 +1088,7 @@ extern "C" int lt_cross_attention_bwd(const lt_cross_attention_desc* d, void* st
     LT_CHECK_ARG(d->dk && d->dv && aligned16(d->dk) && aligned16(d->dv) && strides_ok(d->sdk, d->B, d->Nk, d->Hkv) && strides_ok(d->sdv, d->B, d->Nk, d->Hkv),
                  "lt_cross_attention_bwd: dk, dv: missing, or pointer or strides not 16-byte aligned");
   a.dout = (const uint16_t*)d->dout; a.dq = (uint16_t*)d->dq; a.dk = (uint16_t*)d->dk; a.dv = (uint16_t*)d->dv;
-  a.sdo = st3(d->sdo); a.sdq = st3(d->sdq); a.sdk = st3(d->sdk); a.sdv = st3(d->sdv);
+  a.sdo = st3(d->sdo, d->Nq); a.sdq = st3(d->sdq, d->Nq); a.sdk = st3(d->sdk, d->Nk); a.sdv = st3(d->sdv, d->Nk);
   if (d->Nq == 0) {   // no queries: the keys' gradients are zero
     if (d->Nk > 0) {
       const int64_t n = (int64_t)a.B * a.Nk * a.Hkv * (a.dh / 8);
