@@ -11,8 +11,7 @@
 //   forward   S^T = K Q^T  (lane -> query)  ->  O^T  = V^T P^T      softmax statistics are per lane + one exchange between the wave's halves
 //   dQ        S^T, dP^T = V dO^T            ->  dQ^T = K^T dS^T
 //   dK / dV   S = Q K^T, dP = dO V^T (lane -> key)  ->  dV^T = dO^T P, dK^T = Q^T dS
-// Operands whose contraction index is the token index are read from LDS through ds_read_b64_tr_b16 ("T image": [4 tokens][16 d] pieces of 128 B),
-// the others from padded rows (stride 2 * 32 HD + 16 B: 16 consecutive rows land on 16 different 16-byte bank groups).
+// One LDS image of a token chunk serves both kinds of operand: rows of d, and (ds_read_b64_tr_b16) columns whose contraction index is the token.
 // Keys that are not visible are staged as zeros (what the caller's padding holds is never multiplied) and their scores start at -inf.
 #include "lt_common.h"
 
@@ -82,23 +81,30 @@ __device__ __forceinline__ s16x8 ld8(const uint16_t* p, bool ok) {
 }
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); __builtin_amdgcn_wave_barrier(); }   // lgkmcnt(0)
 
-// ---- LDS images ------------------------------------------------------------------------------------------------------------------
-template <int HD> constexpr int row_stride() { return HD * 64 + 16; }
-template <int HD> __device__ __forceinline__ s16x8 row_frag(const char* img, int tile, int ks) {
-  const int l = lane();
-  return *reinterpret_cast<const s16x8*>(img + (tile * 32 + (l & 31)) * row_stride<HD>() + (2 * ks + (l >> 5)) * 16);
+// ---- the LDS image -----------------------------------------------------------------------------------------------------------------
+// T tokens x 32 HD columns of 16 bits as [4 tokens][16 d] pieces of 128 B, read both ways: rows of 8 consecutive d (ds_read_b128) and, for products
+// over the token index, transposed (ds_read_b64_tr_b16 takes one piece per 16 lanes).  Piece (q = token / 4, b = d / 16) lies at
+// q * 2 HD + (b ^ (q & 1)); its token rows are rotated by b and their two 16-byte halves swapped where q & 2: the 16 rows that one phase of a
+// ds_read_b128 touches land on 16 different bank groups, and so do the 16-byte stores of a staged row.
+template <int HD> __device__ __forceinline__ int img_off(int r, int c) {   // 16-byte chunk c of token r
+  const int q = r >> 2, b = c >> 1;
+  return (q * (2 * HD) + (b ^ (q & 1))) * 128 + ((((r & 3) + b) & 3) << 5) + (((c ^ (q >> 1)) & 1) << 4);
 }
-template <int HD> __device__ __forceinline__ int tr_off(int r, int c) {   // 16-byte chunk c of token r in the T image
-  return ((r >> 2) * (2 * HD) + (c >> 1)) * 128 + ((((r & 3) + (c >> 1)) & 3) << 5) + ((c & 1) << 4);
+template <int HD> __device__ __forceinline__ s16x8 row_frag(const char* img, int tile, int ks) {   // 32 tokens x 16 d
+  const int l = lane(), r = l & 31, q = r >> 2;
+  const int at = q * (2 * HD * 128) + (((ks & 3) ^ (q & 1)) << 7) + ((((r & 3) + ks) & 3) << 5) + ((((l >> 5) ^ (q >> 1)) & 1) << 4);
+  return *reinterpret_cast<const s16x8*>(img + at + tile * (8 * 2 * HD * 128) + (ks >> 2) * 512);
 }
 // rows = 32 d (block db), k-slots = 16 tokens from tok16 (a multiple of 16) in the C-layout slot order
 template <int HD> __device__ __forceinline__ s16x8 tr_frag(const char* img, int db, int tok16) {
-  const int l = lane(), i = l & 15, b = db * 2 + ((l >> 4) & 1), hi = l >> 5;
-  const int inner = ((((i >> 2) + b) & 3) << 5) + ((i & 3) << 3), q = (tok16 >> 2) + hi;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(img + (q * 2 * HD + b) * 128 + inner));
-  const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(img + ((q + 2) * 2 * HD + b) * 128 + inner));
+  const int l = lane(), i = l & 15, cb = (l >> 4) & 1, hi = l >> 5;
+  const int at = hi * (2 * HD * 128) + ((cb ^ hi) << 7) + ((((i >> 2) + cb + 2 * (db & 1)) & 3) << 5);
+  const char* p = img + (tok16 >> 2) * (2 * HD * 128) + db * 256;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + at + ((i & 3) << 3)));
+  const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 2 * (2 * HD * 128) + at + (((i & 3) ^ 2) << 3)));
   return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+template <int HD> constexpr int img_bytes() { return KC * HD * 64; }
 // KC tokens between memory and the images, through registers (the next chunk's loads stay in flight while a chunk is computed).  The loads go through
 // a buffer descriptor that begins at the chunk's first token: a thread's offsets are the same for every chunk, no address arithmetic is left to
 // the vector units (it was half of their instructions), and tokens past the end, or columns past head_dim, read as zeros.
@@ -152,18 +158,11 @@ template <int HD> struct Chunk {
     for (int i = 0; i < PER; ++i)
       if (!m[i]) u[i] = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void store_rows(char* img) const {
+  __device__ __forceinline__ void store(char* img) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR;
-      *reinterpret_cast<uint4*>(img + r * row_stride<HD>() + c * 16) = u[i];
-    }
-  }
-  __device__ __forceinline__ void store_tr(char* img) const {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int idx = threadIdx.x + NT * i, r = idx / CPR, c = idx % CPR;
-      *reinterpret_cast<uint4*>(img + tr_off<HD>(r, c)) = u[i];
+      const int idx = threadIdx.x + NT * i;
+      *reinterpret_cast<uint4*>(img + img_off<HD>(idx / CPR, idx % CPR)) = u[i];
     }
   }
 };
@@ -197,8 +196,6 @@ template <int HD> struct KeyChunk {
     return mb ? 0.f : -INFINITY;
   }
 };
-template <int HD> constexpr int row_img() { return KC * row_stride<HD>(); }
-template <int HD> constexpr int tr_img() { return KC * HD * 64; }
 
 // the workgroups of one (batch entry, key head) land on one XCD (workgroup i runs on XCD i % 8): they share its K / V in that L2
 __device__ __forceinline__ bool my_item(const XArgs& a, int per, int& bh, int& item) {
@@ -270,8 +267,8 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
 // Tiled forward: a workgroup owns 4 waves x QT x 32 query rows of one (batch entry, key head) and walks its share of the keys in chunks of 64.
 template <bool F16, int HD, int QT>
 __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
-  __shared__ __attribute__((aligned(16))) char smem[2 * (row_img<HD>() + tr_img<HD>() + KC * 4)];
-  constexpr int BUF = row_img<HD>() + tr_img<HD>() + KC * 4;
+  __shared__ __attribute__((aligned(16))) char smem[2 * (2 * img_bytes<HD>() + KC * 4)];
+  constexpr int BUF = 2 * img_bytes<HD>() + KC * 4;
   int bh, item;
   if (!my_item(a, a.tiles * a.splits, bh, item)) return;
   const int b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, split = item / a.tiles;
@@ -287,9 +284,9 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
   auto load = [&](int c) { in.load(a, kb, vb, mask, c, kend); };
   auto store = [&](int buf) {
     const float bias = in.hide(mask);
-    in.k.store_rows(smem + buf * BUF);
-    in.v.store_tr(smem + buf * BUF + row_img<HD>());
-    if (threadIdx.x < KC) *reinterpret_cast<float*>(smem + buf * BUF + row_img<HD>() + tr_img<HD>() + threadIdx.x * 4) = bias;
+    in.k.store(smem + buf * BUF);
+    in.v.store(smem + buf * BUF + img_bytes<HD>());
+    if (threadIdx.x < KC) *reinterpret_cast<float*>(smem + buf * BUF + 2 * img_bytes<HD>() + threadIdx.x * 4) = bias;
   };
   if (c_lo < c_hi) load(c_lo);
   s16x8 qf[QT][2 * HD];
@@ -315,8 +312,8 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
     const bool more = ch + 1 < c_hi;
     if (more) load(ch + 1);
     const char* K = smem + buf * BUF;
-    const char* V = K + row_img<HD>();
-    const float* bs = reinterpret_cast<const float*>(V + tr_img<HD>());
+    const char* V = K + img_bytes<HD>();
+    const float* bs = reinterpret_cast<const float*>(V + img_bytes<HD>());
     if (row0 < a.R) {
       const bool biased = mask || (ch + 1) * KC > kend;
       f32x16 s[QT][2];
@@ -376,7 +373,7 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
 }
 
 // Few rows (R <= 32: pooling by one query, one new token): the waves share the one row tile and split the KEYS.  K fragments are rows and come
-// straight from memory, V passes through a wave-private T image; the next tile's loads are in flight while a tile is computed.  Bound by reading
+// straight from memory, V passes through a wave-private image; the next tile's loads are in flight while a tile is computed.  Bound by reading
 // K / V: the padded matrix work of a 32-key tile (8 HD MFMAs) hides under its 8 KiB * HD / 2 of loads.
 template <int HD> struct KeyTile {
   s16x8 f[2 * HD];
@@ -390,10 +387,10 @@ template <int HD> struct KeyTile {
     for (int ks = 0; ks < 2 * HD; ++ks)
       if (!ok) f[ks] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
-  __device__ __forceinline__ void store_tr(char* img) const {   // token l % 32, chunk 2 ks + hi
+  __device__ __forceinline__ void store(char* img) const {   // token l % 32, chunk 2 ks + hi
     const int l = lane();
 #pragma unroll
-    for (int ks = 0; ks < 2 * HD; ++ks) *reinterpret_cast<s16x8*>(img + tr_off<HD>(l & 31, 2 * ks + (l >> 5))) = f[ks];
+    for (int ks = 0; ks < 2 * HD; ++ks) *reinterpret_cast<s16x8*>(img + img_off<HD>(l & 31, 2 * ks + (l >> 5))) = f[ks];
   }
 };
 
@@ -445,7 +442,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
     }
 #pragma unroll
     for (int ks = 0; ks < 2 * HD; ++ks) s[0] = mma<F16>(kf.f[ks], qf[ks], s[0]);
-    vf.store_tr(img);
+    vf.store(img);
     load(t + 4);
     soft_step<HD, 1>(s, c, m, lsum, o);
     const s16x8 p0 = pack8<F16>(s[0], 0), p1 = pack8<F16>(s[0], 8);
@@ -530,7 +527,7 @@ __device__ __forceinline__ float row_start(float lse, float scale) { return lse 
 // dQ: a workgroup owns 128 query rows and walks its share of the keys; D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
 template <bool F16, int HD>
 __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
-  constexpr int BUF = 2 * row_img<HD>() + tr_img<HD>() + KC * 4;
+  constexpr int BUF = 2 * img_bytes<HD>() + KC * 4;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   int bh, item;
   if (!my_item(a, a.tiles * a.splits, bh, item)) return;
@@ -547,10 +544,9 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
   auto store = [&](int buf) {
     char* p = smem + buf * BUF;
     const float bias = in.hide(mask);
-    in.k.store_rows(p);
-    in.v.store_rows(p + row_img<HD>());
-    in.k.store_tr(p + 2 * row_img<HD>());
-    if (threadIdx.x < KC) *reinterpret_cast<float*>(p + 2 * row_img<HD>() + tr_img<HD>() + threadIdx.x * 4) = bias;
+    in.k.store(p);
+    in.v.store(p + img_bytes<HD>());
+    if (threadIdx.x < KC) *reinterpret_cast<float*>(p + 2 * img_bytes<HD>() + threadIdx.x * 4) = bias;
   };
   if (c_lo < c_hi) load(c_lo);
   const int row0 = (tile * 4 + wave) * 32, r = row0 + (l & 31), g = r / a.Nq, n = r - g * a.Nq;
@@ -582,9 +578,8 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
     const bool more = ch + 1 < c_hi;
     if (more) load(ch + 1);
     const char* K = smem + buf * BUF;
-    const char* V = K + row_img<HD>();
-    const char* Kt = V + row_img<HD>();
-    const float* bs = reinterpret_cast<const float*>(Kt + tr_img<HD>());
+    const char* V = K + img_bytes<HD>();
+    const float* bs = reinterpret_cast<const float*>(V + img_bytes<HD>());
     if (row0 < a.R) {
       const bool biased = mask || (ch + 1) * KC > kend;
 #pragma unroll
@@ -607,8 +602,8 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
         const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
         for (int db = 0; db < HD; ++db) {
-          dq[db] = mma<F16>(tr_frag<HD>(Kt, db, t * 32), d0, dq[db]);
-          dq[db] = mma<F16>(tr_frag<HD>(Kt, db, t * 32 + 16), d1, dq[db]);
+          dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32), d0, dq[db]);
+          dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32 + 16), d1, dq[db]);
         }
       }
     }
@@ -623,8 +618,8 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
 // dK / dV: a wave owns 32 keys (K, V fragments and both accumulators in registers), the query rows pass through LDS in chunks of 64.
 template <bool F16, int HD>
 __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const XArgs a) {
-  constexpr int BUF = 2 * row_img<HD>() + 2 * tr_img<HD>() + 2 * KC * 4;
-  __shared__ __attribute__((aligned(16))) char smem[BUF];
+  constexpr int BUF = 2 * img_bytes<HD>() + 2 * KC * 4;
+  __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   int bh, item;
   if (!my_item(a, a.tiles * a.splits, bh, item)) return;
   const int b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, split = item / a.tiles;
@@ -651,15 +646,14 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
       d_reg = r < a.R ? -a.delta[(int64_t)bh * a.R + r] : 0.f;
     }
   };
-  auto store = [&]() {
-    char* p = smem;
-    qr.store_rows(p); p += row_img<HD>();
-    dr.store_rows(p); p += row_img<HD>();
-    qr.store_tr(p); p += tr_img<HD>();
-    dr.store_tr(p); p += tr_img<HD>();
+  auto store = [&](int buf) {
+    char* p = smem + buf * BUF;
+    qr.store(p);
+    dr.store(p + img_bytes<HD>());
     if (threadIdx.x < KC) {
-      reinterpret_cast<float*>(p)[threadIdx.x] = l_reg;
-      reinterpret_cast<float*>(p)[KC + threadIdx.x] = d_reg;
+      float* st = reinterpret_cast<float*>(p + 2 * img_bytes<HD>());
+      st[threadIdx.x] = l_reg;
+      st[KC + threadIdx.x] = d_reg;
     }
   };
   if (c_lo < c_hi) load(c_lo);
@@ -671,17 +665,16 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
   for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
   const float c = a.scale * LOG2E;
   const bool any = __builtin_amdgcn_ballot_w64(seen) != 0;
+  if (c_lo < c_hi) store(0);
+  __syncthreads();
   for (int ch = c_lo; ch < c_hi; ++ch) {
-    if (ch > c_lo) __syncthreads();
-    store();
-    __syncthreads();
-    if (ch + 1 < c_hi) load(ch + 1);
-    if (!any) continue;
-    const char* Q = smem;
-    const char* O = Q + row_img<HD>();
-    const char* Qt = O + row_img<HD>();
-    const char* Ot = Qt + tr_img<HD>();
-    const float* st = reinterpret_cast<const float*>(Ot + tr_img<HD>());
+    const int buf = (ch - c_lo) & 1;
+    const bool more = ch + 1 < c_hi;
+    if (more) load(ch + 1);
+    const char* Q = smem + buf * BUF;
+    const char* O = Q + img_bytes<HD>();
+    const float* st = reinterpret_cast<const float*>(O + img_bytes<HD>());
+    if (any) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x16 s, dp;
@@ -706,12 +699,15 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
       const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8), d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
       for (int db = 0; db < HD; ++db) {
-        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, t * 32), p0, dv[db]);
-        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, t * 32 + 16), p1, dv[db]);
-        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, t * 32), d0, dk[db]);
-        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, t * 32 + 16), d1, dk[db]);
+        dv[db] = mma<F16>(tr_frag<HD>(O, db, t * 32), p0, dv[db]);
+        dv[db] = mma<F16>(tr_frag<HD>(O, db, t * 32 + 16), p1, dv[db]);
+        dk[db] = mma<F16>(tr_frag<HD>(Q, db, t * 32), d0, dk[db]);
+        dk[db] = mma<F16>(tr_frag<HD>(Q, db, t * 32 + 16), d1, dk[db]);
       }
     }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
   }
   if (key >= a.Nk) return;
   if (!seen) {   // gradients of keys that are not visible are zero whatever dO holds
@@ -780,8 +776,8 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
   D = half_sum(D);
   const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
   if (wave == 0) {
-    q.store_tr(Qt);
-    d.store_tr(Ot);
+    q.store(Qt);
+    d.store(Ot);
     if (hi == 0) { st[r] = s0; st[32 + r] = -D; }
   }
   f32x16 dq[HD];
@@ -797,7 +793,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
       vf.hide(seen);
     }
     load(t + 4);
-    kf.store_tr(Kt);
+    kf.store(Kt);
     f32x16 dk[HD], dv[HD];
     {
       f32x16 s, dp;   // lane -> key
