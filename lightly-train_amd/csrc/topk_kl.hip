@@ -4,15 +4,19 @@
 //   p_j = exp(t_j / T - t_lse), and everything else is one bucket, p_rest = max(0, 1 - sum p_j) against q_rest = sum of q over the classes not kept.
 //   loss = w (sum_j p_j (log p_j - log q_j) + p_rest (log p_rest - log q_rest)),   w = coef * row_weight
 //   dlogits = w / T * { q_j - p_j  kept;  q_i (1 - p_rest / q_rest)  others }
-// Bound by memory: the row is read once and its gradient written once.  A row of up to 64 elements (128 of 16 bits) per thread of one workgroup stays
-// in registers between the passes over it (maximum, sum of exponentials, gradient); longer rows are read three times, through the caches.
+// Bound by memory: the row is read once and its gradient written once.  Up to 96 registers of a thread hold its part of the row between the three passes
+// over it (maximum, sum of exponentials, gradient), what does not fit is read again, through the caches: two workgroups of 512 threads to a
+// CU, so that one's stores run under the other's loads, beat one of 1024 that holds a row of 65 536 fp32 whole.
 // The classes not kept are summed on their own (a bitmap in LDS says which are) against their own maximum: q_rest as 1 - sum of the kept q would
 // cancel, and p_rest is formed in 64 bits for the same reason.  The kept classes' gradients overwrite the row's after a barrier.
 #include "lt_common.h"
 
 namespace {
 
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int CUS = 256;
 constexpr int MAX_K = 1024;         // kept entries of a row
 constexpr int MAX_CLASSES = 1 << 18;   // (their bitmap and the kept entries fit 64 KiB of LDS)
 
@@ -36,20 +40,64 @@ template <> __device__ __forceinline__ bf_t putf<bf_t>(float x) { return {f2bf(x
 template <> __device__ __forceinline__ hf_t putf<hf_t>(float x) { return {__builtin_bit_cast(uint16_t, (_Float16)x)}; }
 template <typename T, int E> struct alignas(E * sizeof(T)) Pack { T v[E]; };
 
+// A row behind a buffer descriptor: what lies past its end reads as zeros and is not written, and no lane needs a condition or a 64-bit address.
+struct Row {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Row(const void* p, uint32_t bytes) {
+    const uint64_t u = (uint64_t)p;
+    const uint64_t q = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u) |
+                       ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32)) << 32);
+    r = __builtin_amdgcn_make_buffer_rsrc((void*)q, 0, (int)bytes, 0x00020000);
+  }
+  template <typename P> __device__ __forceinline__ P get(int off) const {
+    if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    else if constexpr (sizeof(P) == 4) return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    else return __builtin_bit_cast(P, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+  }
+  template <typename P> __device__ __forceinline__ void put(int off, const P& x) const {
+    if constexpr (sizeof(P) == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, x), r, off, 0, 0);
+    else if constexpr (sizeof(P) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, x), r, off, 0, 0);
+    else if constexpr (sizeof(P) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), r, off, 0, 0);
+  }
+};
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-__device__ __forceinline__ double block_sum_d(double v, double* red) {
-  v = wave_sum_d(v);
+// three maxima and a count over the workgroup, one pair of barriers
+__device__ __forceinline__ void block_max3_sum(float& x, float& y, float& z, int n, float* red, int& total) {
+  x = wave_max(x);
+  y = wave_max(y);
+  z = wave_max(z);
+  float f = wave_sum((float)n);     // <= 1024: exact
   const int w = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
+  float4* r = reinterpret_cast<float4*>(red);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[w] = v;
+  if ((threadIdx.x & 63) == 0) r[w] = make_float4(x, y, z, f);
   __syncthreads();
-  double s = 0.0;
-  for (int i = 0; i < nw; ++i) s += red[i];
-  return s;
+  float4 a = r[0];
+  for (int i = 1; i < nw; ++i) { const float4 b = r[i]; a = make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), a.w + b.w); }
+  x = a.x; y = a.y; z = a.z;
+  total = (int)a.w;
+}
+// three sums and, when asked, one in 64 bits
+__device__ __forceinline__ void block_sum3(float& x, float& y, float& z, double& p, float* red, double* redd, bool with_p) {
+  x = wave_sum(x);
+  y = wave_sum(y);
+  z = wave_sum(z);
+  if (with_p) p = wave_sum_d(p);
+  const int w = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
+  float4* r = reinterpret_cast<float4*>(red);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) { r[w] = make_float4(x, y, z, 0.f); redd[w] = p; }
+  __syncthreads();
+  float4 a = r[0];
+  double q = redd[0];
+  for (int i = 1; i < nw; ++i) { const float4 b = r[i]; a.x += b.x; a.y += b.y; a.z += b.z; q += redd[i]; }
+  x = a.x; y = a.y; z = a.z;
+  p = q;
 }
 __device__ __forceinline__ float teacher_value(const TopkArgs& a, int64_t row, int j) {
   const int64_t at = row * a.ldv + j;
@@ -63,160 +111,191 @@ __device__ __forceinline__ int teacher_class(const TopkArgs& a, int64_t row, int
   return c >= 0 && c < a.K ? (int)c : -1;
 }
 
-// NV chunks of E elements per thread, chunk i of thread t at element (i * blockDim + t) * E.  KEEP: they stay in registers; otherwise NV is ignored and
-// every pass reads the row again.
-template <typename TS, typename TD, int E, int NV, bool KEEP>
-__global__ __launch_bounds__(1024) void topk_kl_kernel(const TopkArgs a) {
-  extern __shared__ uint32_t dyn[];       // [ceil(K / 32)] kept bits | [k] class | [k] probability
-  __shared__ float red[32];
+// Chunk i of thread t: E elements at (i * blockDim + t) * E.  The first NV chunks of a thread stay in registers, any further ones are read again in
+// every pass.  A workgroup walks rows blockIdx.x, + gridDim.x, ...: the next row's chunk is requested right behind the store of the chunk that held its
+// registers, its kept entries ahead of that.
+constexpr int EPT = 2;   // kept entries per thread that are requested ahead (all of them: k <= 1024, and workgroups that walk rows have 512 threads)
+template <typename TS, typename TD, int E, int NV, int NTMAX>
+__global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
+  extern __shared__ uint32_t dyn[];       // [ceil(max(K, NV * blockDim * E) / 32)] kept bits (set past K) | [k] class | [k] value, then probability | [k] student logit
+  __shared__ __attribute__((aligned(16))) float red[64];
   __shared__ double redd[16];
   __shared__ int twice;
-  const int nt = blockDim.x, words = (a.K + 31) >> 5;
+  const int nt = blockDim.x, words = (max(a.K, NV * nt * E) + 31) >> 5;
   uint32_t* bits = dyn;
   int* cls = reinterpret_cast<int*>(dyn + words);
-  float* prob = reinterpret_cast<float*>(cls + a.k);
-  const int64_t row = blockIdx.x;
-  const TS* s = static_cast<const TS*>(a.s) + row * a.ld;
-  TD* d = static_cast<TD*>(a.d) + row * a.ldd;
-  const float w = a.coef * (a.row_weight ? a.row_weight[row] : 1.f), c = a.inv_temp * LOG2E;
+  float* val = reinterpret_cast<float*>(cls + a.k);
+  float* zs = val + a.k;
   const int chunks = (a.K + E - 1) / E;
+  const float c = a.inv_temp * LOG2E;
   typedef Pack<TS, E> PS;
   typedef Pack<TD, E> PD;
 
-  PS v[KEEP ? NV : 1];
-  if constexpr (KEEP) {
+  PS v[NV];
+  int at = threadIdx.x;      // (opaque to the compiler in every row: it would otherwise keep one offset per chunk alive through the loop)
+  auto load = [&](const Row& s, int i) { v[i] = s.get<PS>((at + i * nt) * (int)sizeof(PS)); };
+  // entry j of a row: class and teacher value, then the student's logit there
+  int ecls[EPT];
+  float eval[EPT], ez[EPT];
+  auto entries = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int j = i * nt + threadIdx.x;
+      ecls[i] = j < a.k ? teacher_class(a, row, j) : -1;
+      eval[i] = j < a.k ? teacher_value(a, row, j) : 0.f;
+    }
+  };
+  auto gather = [&](const TS* s) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) ez[i] = ecls[i] >= 0 ? getf(s[ecls[i]]) : 0.f;
+  };
+  for (int i = threadIdx.x; i < words; i += nt) bits[i] = i * 32 >= a.K ? 0xffffffffu : a.K - i * 32 >= 32 ? 0u : 0xffffffffu << (a.K - i * 32);
+  if (threadIdx.x == 0) twice = 0;
+  int64_t row = blockIdx.x;
+  entries(row);
+  gather(static_cast<const TS*>(a.s) + row * a.ld);
+  {
+    const Row r(static_cast<const TS*>(a.s) + row * a.ld, a.K * sizeof(TS));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load(r, i);
+  }
+  __syncthreads();
+
+  for (; row < a.rows; row += gridDim.x) {
+    asm volatile("" : "+v"(at));
+    const TS* s = static_cast<const TS*>(a.s) + row * a.ld;
+    TD* d = static_cast<TD*>(a.d) + row * a.ldd;
+    const bool more = row + gridDim.x < a.rows;
+    const TS* sn = s + (more ? (int64_t)gridDim.x * a.ld : 0);
+    const Row rn(sn, more ? a.K * sizeof(TS) : 0), rd(d, a.d ? a.K * sizeof(TD) : 0);
+    const float w = a.coef * (a.row_weight ? a.row_weight[row] : 1.f);
+    // ---- the kept entries into LDS
+    auto keep = [&](int j, int x, float t, float z) {
+      cls[j] = x;
+      val[j] = t;
+      zs[j] = z;
+      if (x >= 0 && (atomicOr(&bits[x >> 5], 1u << (x & 31)) >> (x & 31)) & 1) twice = 1;
+    };
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (i * nt + (int)threadIdx.x < a.k) keep(i * nt + threadIdx.x, ecls[i], eval[i], ez[i]);
+    for (int j = EPT * nt + threadIdx.x; j < a.k; j += nt) {
+      const int x = teacher_class(a, row, j);
+      keep(j, x, teacher_value(a, row, j), x >= 0 ? getf(s[x]) : 0.f);
+    }
+    if (more) entries(row + gridDim.x);
+    __syncthreads();
+    if (twice) {     // an index again in its row: its first entry counts
+      for (int j = threadIdx.x; j < a.k; j += nt) {
+        const int x = teacher_class(a, row, j);
+        bool again = false;
+        for (int i = 0; i < j && !again; ++i) again = x >= 0 && teacher_class(a, row, i) == x;
+        if (again) cls[j] = -1;
+      }
+      __syncthreads();
+    }
+    float tmax = -INFINITY, zmax = -INFINITY;
+    int mine = 0;
+    for (int j = threadIdx.x; j < a.k; j += nt)
+      if (cls[j] >= 0) {
+        ++mine;
+        tmax = fmaxf(tmax, val[j]);
+        zmax = fmaxf(zmax, zs[j]);
+      }
+    // ---- the student's classes that are not kept: maximum, then the sum of exponentials against it.  A kept class becomes -inf here.
+    auto hide = [&](int ch, PS& x) {
+      const uint32_t m = bits[(ch * E) >> 5] >> ((ch * E) & 31);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if ((m >> e) & 1) x.v[e] = putf<TS>(-INFINITY);
+      }
+    };
+    auto each = [&](auto&& f) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) f(v[i]);
+#pragma unroll 4
+      for (int ch = NV * nt + threadIdx.x; ch < chunks; ch += nt) {
+        PS x = *reinterpret_cast<const PS*>(s + (int64_t)ch * E);
+        hide(ch, x);
+        f(x);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) hide(i * nt + at, v[i]);
+    float mrest = -INFINITY;
+    each([&](const PS& x) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) mrest = fmaxf(mrest, getf(x.v[e]));
+    });
+    int kept;
+    block_max3_sum(tmax, zmax, mrest, mine, red, kept);
+    const bool live = kept > 0 && w != 0.f && (a.t_lse || tmax > -INFINITY);   // otherwise nothing is known of this row, or nothing asked
+    const float mr = mrest == -INFINITY ? 0.f : mrest, m = fmaxf(zmax, mrest);
+    float srest = 0.f, stop = 0.f, tsum = 0.f;
+    double psum = 0.0;
+    // (differences first, then the scale: x c - m c would carry the rounding of m c into every term alike, and so into the loss)
+    each([&](const PS& x) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) srest += __builtin_amdgcn_exp2f((getf(x.v[e]) - mr) * c);
+    });
+    // ---- teacher probabilities and the kept classes' share of the student
+    for (int j = threadIdx.x; j < a.k; j += nt)
+      if (cls[j] >= 0) {
+        const float t = val[j];
+        if (a.t_lse) psum += exp((double)t * (double)a.inv_temp - (double)a.t_lse[row]);
+        else tsum += __expf((t - tmax) * a.inv_temp);
+        stop += __builtin_amdgcn_exp2f((zs[j] - m) * c);
+      }
+    block_sum3(srest, stop, tsum, psum, red, redd, a.t_lse != nullptr);
+    const float rest = a.t_lse && kept < a.K && psum < 1.0 ? (float)(1.0 - psum) : 0.f;
+    const float frest = mrest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mrest - m) * c);
+    const float total = stop + srest * frest, lt = logf(total), ltsum = a.t_lse ? 0.f : logf(tsum);
+    const float g = w * a.inv_temp, gr = g * (frest / total - (srest > 0.f ? rest / srest : 0.f));
+    // ---- loss and gradient
+    float part = 0.f;
+    for (int j = threadIdx.x; j < a.k; j += nt)
+      if (cls[j] >= 0) {
+        const float z = (zs[j] - m) * a.inv_temp;
+        const float logp = a.t_lse ? (float)((double)val[j] * (double)a.inv_temp - (double)a.t_lse[row]) : (val[j] - tmax) * a.inv_temp - ltsum;
+        const float p = a.t_lse ? expf(logp) : __expf((val[j] - tmax) * a.inv_temp) / tsum;
+        if (p > 0.f) part += p * (logp - (z - lt));
+        val[j] = p;
+        zs[j] = __builtin_amdgcn_exp2f((zs[j] - m) * c) / total;
+      }
+    if (more) gather(sn);
+    const float cl = live ? c : 0.f, gl = live ? gr : 0.f, ml = live ? mr : 0.f;
+    auto grad = [&](const PS& x) {
+      PD o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float z = live ? getf(x.v[e]) : 0.f;      // (a row that is not asked for may hold NaN)
+        o.v[e] = putf<TD>(gl * __builtin_amdgcn_exp2f((z - ml) * cl));
+      }
+      return o;
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int ch = i * nt + threadIdx.x;
-      if (ch < chunks) v[i] = *reinterpret_cast<const PS*>(s + (int64_t)ch * E);
+      rd.put((at + i * nt) * (int)sizeof(PD), grad(v[i]));
+      load(rn, i);
     }
-  }
-  // ---- the kept entries
-  for (int i = threadIdx.x; i < words; i += nt) bits[i] = 0;
-  if (threadIdx.x == 0) twice = 0;
-  __syncthreads();
-  for (int j = threadIdx.x; j < a.k; j += nt) {
-    const int x = teacher_class(a, row, j);
-    cls[j] = x;
-    if (x >= 0 && (atomicOr(&bits[x >> 5], 1u << (x & 31)) >> (x & 31)) & 1) twice = 1;
-  }
-  __syncthreads();
-  if (twice) {     // an index again in its row: its first entry counts
+    if (a.d) {
+#pragma unroll 4
+      for (int ch = NV * nt + threadIdx.x; ch < chunks; ch += nt) *reinterpret_cast<PD*>(d + (int64_t)ch * E) = grad(*reinterpret_cast<const PS*>(s + (int64_t)ch * E));
+    }
+    part = block_sum(part, red);     // (its barriers also order the row's stores before the kept classes')
+    if (threadIdx.x == 0) {
+      if (rest > 0.f) part += rest * (logf(rest) - ((mr - m) * a.inv_temp + logf(srest) - lt));   // srest = 0: +inf
+      a.loss_rows[row] = live ? w * part : 0.f;
+      twice = 0;
+    }
     for (int j = threadIdx.x; j < a.k; j += nt) {
-      const int x = teacher_class(a, row, j);
-      bool again = false;
-      for (int i = 0; i < j && !again; ++i) again = x >= 0 && teacher_class(a, row, i) == x;
-      if (again) cls[j] = -1;
+      const int x = cls[j];
+      if (x < 0) continue;
+      atomicAnd(&bits[x >> 5], ~(1u << (x & 31)));
+      if (a.d && live) d[x] = putf<TD>(g * (zs[j] - val[j]));
     }
     __syncthreads();
   }
-  float tmax = -INFINITY, zmax = -INFINITY;
-  int mine = 0;
-  for (int j = threadIdx.x; j < a.k; j += nt)
-    if (cls[j] >= 0) {
-      ++mine;
-      tmax = fmaxf(tmax, teacher_value(a, row, j));
-      zmax = fmaxf(zmax, getf(s[cls[j]]));
-    }
-  const int kept = (int)block_sum((float)mine, red);   // <= 1024: exact
-  tmax = block_max(tmax, red);
-  zmax = block_max(zmax, red);
-  if (kept == 0 || w == 0.f || (!a.t_lse && tmax == -INFINITY)) {   // nothing known of this row, or nothing asked
-    if (threadIdx.x == 0) a.loss_rows[row] = 0.f;
-    if (a.d)
-      for (int ch = threadIdx.x; ch < chunks; ch += nt) {
-        PD o;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = putf<TD>(0.f);
-        *reinterpret_cast<PD*>(d + (int64_t)ch * E) = o;
-      }
-    return;
-  }
-  // ---- the student's classes that are not kept: maximum, then the sum of exponentials against it
-  float mrest = -INFINITY;
-  auto bits_of = [&](int ch) -> uint32_t { return E == 1 ? bits[ch >> 5] >> (ch & 31) : bits[(ch * E) >> 5] >> ((ch * E) & 31); };
-  auto each = [&](auto&& f) {
-    if constexpr (KEEP) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int ch = i * nt + threadIdx.x;
-        if (ch < chunks) f(ch, v[i]);
-      }
-    } else {
-      for (int ch = threadIdx.x; ch < chunks; ch += nt) f(ch, *reinterpret_cast<const PS*>(s + (int64_t)ch * E));
-    }
-  };
-  each([&](int ch, const PS& x) {
-    const uint32_t m = bits_of(ch);
-#pragma unroll
-    for (int e = 0; e < E; ++e) mrest = fmaxf(mrest, (m >> e) & 1 ? -INFINITY : getf(x.v[e]));
-  });
-  mrest = block_max(mrest, red);
-  const float mr = mrest == -INFINITY ? 0.f : mrest, nmr = -mr * c;
-  float srest = 0.f;
-  each([&](int ch, const PS& x) {
-    const uint32_t m = bits_of(ch);
-#pragma unroll
-    for (int e = 0; e < E; ++e) srest += (m >> e) & 1 ? 0.f : __builtin_amdgcn_exp2f(fmaf(getf(x.v[e]), c, nmr));
-  });
-  srest = block_sum(srest, red);
-  // ---- teacher probabilities and the kept classes' share of the student
-  const float m = fmaxf(zmax, mrest);
-  float stop = 0.f, tsum = 0.f;
-  double psum = 0.0;
-  for (int j = threadIdx.x; j < a.k; j += nt) {
-    float p = 0.f;
-    if (cls[j] >= 0) {
-      const float t = teacher_value(a, row, j);
-      if (a.t_lse) {
-        const double pd = exp((double)t * (double)a.inv_temp - (double)a.t_lse[row]);
-        psum += pd;
-        p = (float)pd;
-      } else {
-        p = __expf((t - tmax) * a.inv_temp);
-        tsum += p;
-      }
-      stop += __builtin_amdgcn_exp2f((getf(s[cls[j]]) - m) * c);
-    }
-    prob[j] = p;
-  }
-  stop = block_sum(stop, red);
-  float rest = 0.f, pmul = 1.f;
-  if (a.t_lse) {
-    psum = block_sum_d(psum, redd);
-    rest = kept < a.K && psum < 1.0 ? (float)(1.0 - psum) : 0.f;
-  } else {
-    pmul = 1.f / block_sum(tsum, red);
-  }
-  const float frest = mrest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mrest - m) * c);
-  const float total = stop + srest * frest, lt = __logf(total);
-  float part = 0.f;
-  for (int j = threadIdx.x; j < a.k; j += nt)
-    if (cls[j] >= 0) {
-      const float p = prob[j] * pmul;
-      if (p > 0.f) {
-        const float logp = a.t_lse ? (float)((double)teacher_value(a, row, j) * (double)a.inv_temp - (double)a.t_lse[row])
-                                   : (teacher_value(a, row, j) - tmax) * a.inv_temp + __logf(pmul);
-        part += p * (logp - ((getf(s[cls[j]]) - m) * a.inv_temp - lt));
-      }
-    }
-  part = block_sum(part, red);
-  if (threadIdx.x == 0) {
-    if (rest > 0.f) part += rest * (__logf(rest) - ((mr - m) * a.inv_temp + __logf(srest) - lt));   // srest = 0: +inf
-    a.loss_rows[row] = w * part;
-  }
-  if (!a.d) return;
-  // ---- gradient
-  const float g = w * a.inv_temp, gr = g * (frest / total - (srest > 0.f ? rest / srest : 0.f));
-  each([&](int ch, const PS& x) {
-    PD o;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o.v[e] = putf<TD>(gr * __builtin_amdgcn_exp2f(fmaf(getf(x.v[e]), c, nmr)));
-    *reinterpret_cast<PD*>(d + (int64_t)ch * E) = o;
-  });
-  __syncthreads();
-  for (int j = threadIdx.x; j < a.k; j += nt)
-    if (cls[j] >= 0) d[cls[j]] = putf<TD>(g * (__builtin_amdgcn_exp2f((getf(s[cls[j]]) - m) * c) / total - prob[j] * pmul));
 }
 
 // loss[0] += sum of the rows' losses, in a fixed order
@@ -228,27 +307,23 @@ __global__ __launch_bounds__(256) void topk_loss_kernel(const float* __restrict_
   if (threadIdx.x == 0) loss[0] += s;
 }
 
-template <typename TS, typename TD, int E, int NV, bool KEEP> void go(const TopkArgs& a, int nt, hipStream_t st) {
-  const size_t lds = ((size_t)((a.K + 31) / 32) + 2 * (size_t)a.k) * 4;
-  hipLaunchKernelGGL((topk_kl_kernel<TS, TD, E, NV, KEEP>), dim3(a.rows), dim3(nt), lds, st, a);
-}
-// threads of a workgroup: the fewest waves whose registers hold the row
-int threads_for(int chunks, int nv) {
-  int nt = 64;
-  while (nt < 1024 && (int64_t)nt * nv < chunks) nt *= 2;
-  return nt;
+template <typename TS, typename TD, int E, int NV, int NTMAX> void go(const TopkArgs& a, int grid, hipStream_t st) {
+  const int chunks = lt_cdiv(a.K, E);
+  int nt = 64;                        // the fewest waves whose registers hold the row
+  while (nt < NTMAX && (int64_t)nt * NV < chunks) nt *= 2;
+  const int bits = a.K > NV * nt * E ? a.K : NV * nt * E;
+  const size_t lds = ((size_t)((bits + 31) / 32) + 3 * (size_t)a.k) * 4;
+  hipLaunchKernelGGL((topk_kl_kernel<TS, TD, E, NV, NTMAX>), dim3(grid < a.rows ? grid : a.rows), dim3(nt), lds, st, a);
 }
 template <typename TS, typename TD> void dispatch(const TopkArgs& a, hipStream_t st) {
   constexpr int E = 16 / sizeof(TS);
   const bool vec = a.K % E == 0 && a.ld % E == 0 && ((uintptr_t)a.s & 15) == 0 && (!a.d || (a.ldd % E == 0 && ((uintptr_t)a.d & (E * sizeof(TD) - 1)) == 0));
   if (vec) {
-    const int chunks = a.K / E;
-    if (chunks <= 4 * 1024) go<TS, TD, E, 4, true>(a, threads_for(chunks, 4), st);
-    else if (chunks <= 16 * 1024) go<TS, TD, E, 16, true>(a, threads_for(chunks, 16), st);
-    else go<TS, TD, E, 1, false>(a, 1024, st);
+    if (a.K / E <= 4 * 1024) go<TS, TD, E, 4, 1024>(a, a.rows, st);
+    else go<TS, TD, E, sizeof(TS) == 4 ? 32 : 16, 512>(a, CUS, st);
   } else {   // rows that are not whole 16-byte pieces: one element per lane and load
-    if (a.K <= 16 * 1024) go<TS, TD, 1, 16, true>(a, threads_for(a.K, 16), st);
-    else go<TS, TD, 1, 1, false>(a, 1024, st);
+    if (a.K <= 16 * 1024) go<TS, TD, 1, 16, 1024>(a, a.rows, st);
+    else go<TS, TD, 1, 80, 512>(a, CUS, st);
   }
 }
 
