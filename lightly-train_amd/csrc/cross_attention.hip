@@ -206,18 +206,28 @@ __device__ __forceinline__ bool my_item(const XArgs& a, int per, int& bh, int& i
 }
 __device__ __forceinline__ int key_end(const XArgs& a, int b) { return __builtin_amdgcn_readfirstlane(a.klen ? min(max(a.klen[b], 0), a.Nk) : a.Nk); }
 
-// accumulators acc[HD] in C layout (lane -> row, registers -> d) to 16-bit rows / fp32 partial rows
-template <bool F16, int HD> __device__ __forceinline__ void put_row(uint16_t* dst, const f32x16 (&acc)[HD], float mul, int dh) {
-  const int hi = lane() >> 5;
+// Accumulators acc[HD] in C layout (lane -> row, registers -> d) as 16-bit rows: through 32 rows of an LDS image that belongs to the wave, so that
+// 4 HD neighbouring lanes write one row in 16-byte pieces (written from the registers, a store instruction would touch 32 rows 16 bytes each).
+// at(r): where row r of the tile goes, nullptr = nowhere.
+template <bool F16, int HD, typename At> __device__ __forceinline__ void put_tile(char* img, const f32x16 (&acc)[HD], float mul, int dh, At&& at) {
+  const int l = lane(), hi = l >> 5;
 #pragma unroll
   for (int db = 0; db < HD; ++db)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = db * 32 + 8 * g + 4 * hi;
-      if (d < dh) *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack2<F16>(acc[db][4 * g] * mul, acc[db][4 * g + 1] * mul),
-                                                                  pack2<F16>(acc[db][4 * g + 2] * mul, acc[db][4 * g + 3] * mul));
-    }
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<uint2*>(img + img_off<HD>(l & 31, db * 4 + g) + 8 * hi) =
+          make_uint2(pack2<F16>(acc[db][4 * g] * mul, acc[db][4 * g + 1] * mul), pack2<F16>(acc[db][4 * g + 2] * mul, acc[db][4 * g + 3] * mul));
+  wait_lds();
+#pragma unroll
+  for (int i = 0; i < 2 * HD; ++i) {
+    const int idx = l + 64 * i, r = idx / (4 * HD), c = idx % (4 * HD);
+    const uint4 u = *reinterpret_cast<const uint4*>(img + img_off<HD>(r, c));
+    uint16_t* p = at(r);
+    if (p && c * 8 < dh) *reinterpret_cast<uint4*>(p + c * 8) = u;
+  }
+  wait_lds();
 }
+// ... and as fp32 partial rows, straight from the registers
 template <int HD> __device__ __forceinline__ void put_partial(float* dst, const f32x16 (&acc)[HD], float mul, int dh) {
   const int hi = lane() >> 5;
 #pragma unroll
@@ -357,17 +367,19 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
   }
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const int r = row0 + t * 32 + (l & 31), g = r / a.Nq, n = r - g * a.Nq;
+    const int r = row0 + t * 32 + (l & 31);
     const float ls = half_sum(lsum[t]);
-    if (r >= a.R) continue;
     if (a.splits > 1) {
+      if (r >= a.R) continue;
       const int64_t rows = (int64_t)a.B * a.Hkv * a.R, row = split * rows + (int64_t)bh * a.R + r;
       put_partial<HD>(a.ws + row * a.dh, o[t], 1.f, a.dh);
       if (hi == 0) *reinterpret_cast<float2*>(a.ws + a.splits * rows * a.dh + row * 2) = make_float2(m[t], ls);
     } else {
-      const int h = hk * a.G + g;
-      put_row<F16, HD>(a.out + b * a.so.b + n * a.so.n + h * a.so.h, o[t], ls != 0.f ? 1.f / ls : 0.f, a.dh);
-      if (hi == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + n] = ls != 0.f ? m[t] * a.scale + __logf(ls) : -INFINITY;
+      put_tile<F16, HD>(smem + wave * (32 * HD * 64), o[t], ls != 0.f ? 1.f / ls : 0.f, a.dh, [&](int x) -> uint16_t* {
+        const int rr = row0 + t * 32 + x, g = rr / a.Nq, n = rr - g * a.Nq;
+        return rr < a.R ? a.out + b * a.so.b + n * a.so.n + (int64_t)(hk * a.G + g) * a.so.h : nullptr;
+      });
+      if (hi == 0 && a.lse && r < a.R) a.lse[((int64_t)b * a.H + hk * a.G) * a.Nq + r] = ls != 0.f ? m[t] * a.scale + __logf(ls) : -INFINITY;   // (rows of a group lie one after the other)
     }
   }
 }
@@ -525,8 +537,10 @@ __global__ __launch_bounds__(NT) void xattn_join_kernel(const XArgs a) {
 __device__ __forceinline__ float row_start(float lse, float scale) { return lse == -INFINITY ? -INFINITY : -lse / scale; }
 
 // dQ: a workgroup owns 128 query rows and walks its share of the keys; D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
-template <bool F16, int HD>
-__global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
+// SUMS (at most two chunks of keys): a pass of its own forms D = sum_k P dP from the fp32 products -- rowsum(dO * O) carries the rounding of O, most of
+// dS's error when a row's probabilities are spread over a few keys only.
+template <bool F16, int HD, bool SUMS>
+__global__ __launch_bounds__(NT, HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XArgs a) {
   constexpr int BUF = 2 * img_bytes<HD>() + KC * 4;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   int bh, item;
@@ -566,17 +580,19 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
     for (int j = 0; j < 8; ++j) D = fmaf(to_f<F16>(df[ks][j]), to_f<F16>(of[j]), D);
   }
   D = half_sum(D);
-  if (split == 0 && hi == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = D;
   const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
   f32x16 dq[HD];
 #pragma unroll
   for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
   if (c_lo < c_hi) store(0);
   __syncthreads();
-  for (int ch = c_lo; ch < c_hi; ++ch) {
-    const int buf = (ch - c_lo) & 1;
-    const bool more = ch + 1 < c_hi;
-    if (more) load(ch + 1);
+  const int first = SUMS ? c_hi - c_lo : 0, all = first + c_hi - c_lo;
+  float Dx = 0.f;
+  for (int it = 0; it < all; ++it) {
+    const bool more = it + 1 < all, sums = SUMS && it < first;
+    const int ch = c_lo + (sums || !SUMS ? it : it - first), buf = it & 1;
+    if (more) load(SUMS && it + 1 >= first ? c_lo + it + 1 - first : c_lo + it + 1);
+    if (SUMS && it == first) D = half_sum(Dx);
     const char* K = smem + buf * BUF;
     const char* V = K + img_bytes<HD>();
     const float* bs = reinterpret_cast<const float*>(V + img_bytes<HD>());
@@ -584,7 +600,7 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
       const bool biased = mask || (ch + 1) * KC > kend;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        f32x16 s = splat(s0), dp = splat(-D);
+        f32x16 s = splat(s0), dp = splat(sums ? 0.f : -D);
         if (biased) {
 #pragma unroll
           for (int gq = 0; gq < 4; ++gq) {
@@ -599,6 +615,11 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
+        if (SUMS && sums) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) Dx += dp[e];
+          continue;
+        }
         const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
         for (int db = 0; db < HD; ++db) {
@@ -610,9 +631,15 @@ __global__ __launch_bounds__(NT, 2) void xattn_dq_kernel(const XArgs a) {
     if (more) store(buf ^ 1);
     __syncthreads();
   }
-  if (r >= a.R) return;
-  if (a.splits > 1) put_partial<HD>(a.ws + ((int64_t)split * a.B * a.Hkv * a.R + (int64_t)bh * a.R + r) * a.dh, dq, a.scale, a.dh);
-  else put_row<F16, HD>(a.dq + b * a.sdq.b + n * a.sdq.n + h * a.sdq.h, dq, a.scale, a.dh);
+  if (split == 0 && hi == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = D;
+  if (a.splits > 1) {
+    if (r < a.R) put_partial<HD>(a.ws + ((int64_t)split * a.B * a.Hkv * a.R + (int64_t)bh * a.R + r) * a.dh, dq, a.scale, a.dh);
+    return;
+  }
+  put_tile<F16, HD>(smem + wave * (32 * HD * 64), dq, a.scale, a.dh, [&](int x) -> uint16_t* {
+    const int rr = row0 + x, gg = rr / a.Nq, nn = rr - gg * a.Nq;
+    return rr < a.R ? a.dq + b * a.sdq.b + nn * a.sdq.n + (int64_t)(hk * a.G + gg) * a.sdq.h : nullptr;
+  });
 }
 
 // dK / dV: a wave owns 32 keys (K, V fragments and both accumulators in registers), the query rows pass through LDS in chunks of 64.
@@ -709,20 +736,22 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
     if (more) store(buf ^ 1);
     __syncthreads();
   }
-  if (key >= a.Nk) return;
   if (!seen) {   // gradients of keys that are not visible are zero whatever dO holds
 #pragma unroll
     for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
   }
   const float vmul = F16 ? 1.f / P_UP : 1.f;
   if (a.splits > 1) {
+    if (key >= a.Nk) return;
     const int64_t keys = (int64_t)a.B * a.Hkv * a.Nk, at = split * keys + (int64_t)bh * a.Nk + key;
     put_partial<HD>(a.ws + at * a.dh, dk, a.scale, a.dh);
     put_partial<HD>(a.ws + (a.splits * keys + at) * a.dh, dv, vmul, a.dh);
-  } else {
-    put_row<F16, HD>(a.dk + b * a.sdk.b + key * a.sdk.n + hk * a.sdk.h, dk, a.scale, a.dh);
-    put_row<F16, HD>(a.dv + b * a.sdv.b + key * a.sdv.n + hk * a.sdv.h, dv, vmul, a.dh);
+    return;
   }
+  const int key0 = (tile * 4 + wave) * 32;
+  char* img = smem + wave * (32 * HD * 64);
+  put_tile<F16, HD>(img, dk, a.scale, a.dh, [&](int x) -> uint16_t* { return key0 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(key0 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
+  put_tile<F16, HD>(img, dv, vmul, a.dh, [&](int x) -> uint16_t* { return key0 + x < a.Nk ? a.dv + b * a.sdv.b + (int64_t)(key0 + x) * a.sdv.n + hk * a.sdv.h : nullptr; });
 }
 
 // Few rows (R <= 32): every key tile meets the one row tile once, so dK / dV of the tile are complete at once and all three gradients take ONE pass
@@ -731,7 +760,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
 template <bool F16, int HD>
 __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(const XArgs a) {
   constexpr int IMG = 32 * HD * 64, OST = HD * 32 + 4;
-  constexpr int TAIL = 4 * 32 * OST * 4, HEAD = 6 * IMG + 2 * 32 * 4;
+  constexpr int TAIL = 4 * 32 * OST * 4, HEAD = 6 * IMG + (2 + 4) * 32 * 4;
   __shared__ __attribute__((aligned(16))) char smem[TAIL > HEAD ? TAIL : HEAD];
   int bh, split;
   if (!my_item(a, a.splits, bh, split)) return;
@@ -742,10 +771,10 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
   const uint16_t* kb = a.k + b * a.sk.b + hk * a.sk.h;
   const uint16_t* vb = a.v + b * a.sv.b + hk * a.sv.h;
   const uint8_t* mask = a.kmask ? a.kmask + (int64_t)b * a.Nk : nullptr;
-  char* Qt = smem;
-  char* Ot = smem + IMG;
+  char* Q = smem;
+  char* O = smem + IMG;
   char* Kt = smem + (2 + wave) * IMG;
-  float* st = reinterpret_cast<float*>(smem + 6 * IMG);
+  float* st = reinterpret_cast<float*>(smem + 6 * IMG);   // [32] score starts, [32] -D, [4][32] the waves' shares of D
   KeyTile<HD> kn, vn;
   bool in = false;
   uint8_t mb = 1;
@@ -761,28 +790,60 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
   const int64_t h = hk * a.G + g;
   const float lse = r < a.R ? a.lse[((int64_t)b * a.H + h) * a.Nq + n] : -INFINITY;
   const bool live = lse != -INFINITY;
-  KeyTile<HD> q, d;
+  const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
   float D = 0.f;
+  {
+    KeyTile<HD> q, d;
 #pragma unroll
-  for (int ks = 0; ks < 2 * HD; ++ks) {
-    const int dd = ks * 16 + hi * 8;
-    const bool ok = live && dd < a.dh;
-    q.f[ks] = ld8(a.q + b * a.sq.b + n * a.sq.n + h * a.sq.h + dd, ok);
-    d.f[ks] = ld8(a.dout + b * a.sdo.b + n * a.sdo.n + h * a.sdo.h + dd, ok);
-    const s16x8 of = ld8(a.o + b * a.so.b + n * a.so.n + h * a.so.h + dd, ok);
+    for (int ks = 0; ks < 2 * HD; ++ks) {
+      const int dd = ks * 16 + hi * 8;
+      const bool ok = live && dd < a.dh;
+      q.f[ks] = ld8(a.q + b * a.sq.b + n * a.sq.n + h * a.sq.h + dd, ok);
+      d.f[ks] = ld8(a.dout + b * a.sdo.b + n * a.sdo.n + h * a.sdo.h + dd, ok);
+      const s16x8 of = ld8(a.o + b * a.so.b + n * a.so.n + h * a.so.h + dd, ok);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) D = fmaf(to_f<F16>(d.f[ks][j]), to_f<F16>(of[j]), D);
+      for (int j = 0; j < 8; ++j) D = fmaf(to_f<F16>(d.f[ks][j]), to_f<F16>(of[j]), D);
+    }
+    if (wave == 0) {
+      q.store(Q);
+      d.store(O);
+    }
   }
   D = half_sum(D);
-  const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
-  if (wave == 0) {
-    q.store(Qt);
-    d.store(Ot);
-    if (hi == 0) { st[r] = s0; st[32 + r] = -D; }
-  }
   f32x16 dq[HD];
 #pragma unroll
   for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
+  __syncthreads();
+  auto columns = [&](const KeyTile<HD>& kf, const KeyTile<HD>& vf, uint32_t all, float start, f32x16& s, f32x16& dp) {   // lane -> query
+    s = splat(s0);
+    dp = splat(start);
+    if (all != 0xffffffffu) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = (all >> crow(e, hi)) & 1 ? s[e] : -INFINITY;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) {
+      s = mma<F16>(kf.f[ks], row_frag<HD>(Q, 0, ks), s);
+      dp = mma<F16>(vf.f[ks], row_frag<HD>(O, 0, ks), dp);
+    }
+  };
+  if (a.splits == 1 && tiles <= 4) {
+    // Few keys as well: D = sum_k P dP from the fp32 products instead of rowsum(dO * O), whose rounded O would be most of dS's error when a row's
+    // probabilities are spread over a few keys only.  Every wave holds its one tile.
+    const uint32_t all = (uint32_t)__builtin_amdgcn_ballot_w64(in && mb);
+    kn.hide(in && mb);
+    vn.hide(in && mb);
+    f32x16 s, dp;
+    columns(kn, vn, all, 0.f, s, dp);
+    D = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) D = fmaf(__builtin_amdgcn_exp2f(s[e] * c), dp[e], D);
+    D = half_sum(D);
+    if (hi == 0) st[(2 + wave) * 32 + r] = wave < tiles ? D : 0.f;
+    __syncthreads();
+    D = ((st[2 * 32 + r] + st[3 * 32 + r]) + st[4 * 32 + r]) + st[5 * 32 + r];
+  }
+  if (wave == 0 && hi == 0) { st[r] = s0; st[32 + r] = -D; }
   __syncthreads();
   for (int t = t_lo + wave; t < t_hi; t += 4) {
     KeyTile<HD> kf = kn, vf = vn;
@@ -794,58 +855,11 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
     }
     load(t + 4);
     kf.store(Kt);
-    f32x16 dk[HD], dv[HD];
-    {
-      f32x16 s, dp;   // lane -> key
-#pragma unroll
-      for (int gq = 0; gq < 4; ++gq) {
-        const float4 x = *reinterpret_cast<const float4*>(st + 8 * gq + 4 * hi);
-        const float4 y = *reinterpret_cast<const float4*>(st + 32 + 8 * gq + 4 * hi);
-        s[4 * gq] = seen ? x.x : -INFINITY; s[4 * gq + 1] = seen ? x.y : -INFINITY; s[4 * gq + 2] = seen ? x.z : -INFINITY; s[4 * gq + 3] = seen ? x.w : -INFINITY;
-        dp[4 * gq] = y.x; dp[4 * gq + 1] = y.y; dp[4 * gq + 2] = y.z; dp[4 * gq + 3] = y.w;
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2 * HD; ++ks) {
-        s = mma<F16>(q.f[ks], kf.f[ks], s);
-        dp = mma<F16>(d.f[ks], vf.f[ks], dp);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[e] * c);
-        dp[e] *= p;
-        s[e] = F16 ? p * P_UP : p;
-      }
-      const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8), d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
-#pragma unroll
-      for (int db = 0; db < HD; ++db) {
-        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, 0), p0, splat(0.f));
-        dv[db] = mma<F16>(tr_frag<HD>(Ot, db, 16), p1, dv[db]);
-        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, 0), d0, splat(0.f));
-        dk[db] = mma<F16>(tr_frag<HD>(Qt, db, 16), d1, dk[db]);
-      }
-    }
-    const int key = t * 32 + (l & 31);
-    if (key < a.Nk) {
-      if (!seen) {
-#pragma unroll
-        for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
-      }
-      put_row<F16, HD>(a.dk + b * a.sdk.b + key * a.sdk.n + hk * a.sdk.h, dk, a.scale, a.dh);
-      put_row<F16, HD>(a.dv + b * a.sdv.b + key * a.sdv.n + hk * a.sdv.h, dv, F16 ? 1.f / P_UP : 1.f, a.dh);
-    }
-    f32x16 s = splat(s0), dp = splat(-D);   // lane -> query
-    if (all != 0xffffffffu) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = (all >> crow(e, hi)) & 1 ? s[e] : -INFINITY;
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2 * HD; ++ks) {
-      s = mma<F16>(kf.f[ks], q.f[ks], s);
-      dp = mma<F16>(vf.f[ks], d.f[ks], dp);
-    }
+    f32x16 s, dp;
+    columns(kf, vf, all, -D, s, dp);
 #pragma unroll
     for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
-    const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
+    s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
     wait_lds();
 #pragma unroll
     for (int db = 0; db < HD; ++db) {
@@ -853,6 +867,44 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
       dq[db] = mma<F16>(tr_frag<HD>(Kt, db, 16), d1, dq[db]);
     }
     wait_lds();
+    // lane -> key
+#pragma unroll
+    for (int gq = 0; gq < 4; ++gq) {
+      const float4 x = *reinterpret_cast<const float4*>(st + 8 * gq + 4 * hi);
+      const float4 y = *reinterpret_cast<const float4*>(st + 32 + 8 * gq + 4 * hi);
+      s[4 * gq] = x.x; s[4 * gq + 1] = x.y; s[4 * gq + 2] = x.z; s[4 * gq + 3] = x.w;
+      dp[4 * gq] = y.x; dp[4 * gq + 1] = y.y; dp[4 * gq + 2] = y.z; dp[4 * gq + 3] = y.w;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2 * HD; ++ks) {
+      s = mma<F16>(row_frag<HD>(Q, 0, ks), kf.f[ks], s);
+      dp = mma<F16>(row_frag<HD>(O, 0, ks), vf.f[ks], dp);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p = __builtin_amdgcn_exp2f(s[e] * c);   // (a hidden key's column is replaced by zeros below)
+      dp[e] *= p;
+      s[e] = F16 ? p * P_UP : p;
+    }
+    d0 = pack8<F16>(dp, 0);
+    d1 = pack8<F16>(dp, 8);
+    const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8);
+    f32x16 acc[HD];
+#pragma unroll
+    for (int db = 0; db < HD; ++db) {
+      acc[db] = mma<F16>(tr_frag<HD>(Q, db, 0), d0, splat(0.f));
+      acc[db] = mma<F16>(tr_frag<HD>(Q, db, 16), d1, acc[db]);
+      if (!seen) acc[db] = splat(0.f);   // whatever dO holds
+    }
+    put_tile<F16, HD>(Kt, acc, a.scale, a.dh, [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(t * 32 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
+#pragma unroll
+    for (int db = 0; db < HD; ++db) {
+      acc[db] = mma<F16>(tr_frag<HD>(O, db, 0), p0, splat(0.f));
+      acc[db] = mma<F16>(tr_frag<HD>(O, db, 16), p1, acc[db]);
+      if (!seen) acc[db] = splat(0.f);
+    }
+    put_tile<F16, HD>(Kt, acc, F16 ? 1.f / P_UP : 1.f, a.dh,
+                      [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dv + b * a.sdv.b + (int64_t)(t * 32 + x) * a.sdv.n + hk * a.sdv.h : nullptr; });
   }
   __syncthreads();   // images -> the waves' partial dQ rows
   if (r < a.R) put_partial<HD>(reinterpret_cast<float*>(smem) + (wave * 32 + r) * OST, dq, a.scale, HD * 32);
@@ -1023,7 +1075,8 @@ template <bool F16> void run_bwd(XArgs a, float* ws, void* stream) {
   a.delta = ws;
   a.ws = p.few ? ws : ws + delta_floats(a.B, a.R, a.Hkv);
   if (p.few) { XA_HD(xattn_bwd_few_kernel, (unsigned)(bh8 * a.splits), F16) }
-  else { XA_HD(xattn_dq_kernel, (unsigned)(bh8 * a.tiles * a.splits), F16) }
+  else if (a.splits == 1 && a.Nk <= 2 * KC) { XA_HD(xattn_dq_kernel, (unsigned)(bh8 * a.tiles), F16, , true) }
+  else { XA_HD(xattn_dq_kernel, (unsigned)(bh8 * a.tiles * a.splits), F16, , false) }
   if (a.splits > 1) add_splits<F16>(a, a.ws, a.dq, a.sdq, rows, a.R, a.Nq, a.G, stream);
   if (p.few || a.Nk == 0) return;
   p = dkdv_plan(a.B, a.R, a.Nk, a.Hkv, a.dh);
