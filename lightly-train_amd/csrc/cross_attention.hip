@@ -265,9 +265,13 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
 #pragma unroll
   for (int t = 0; t < NK; ++t)
 #pragma unroll
+    for (int e = 0; e < 16; ++e) s[t][e] = fmaf(s[t][e], c, nmc);
+#pragma unroll
+  for (int t = 0; t < NK; ++t)
+#pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c, nmc));
-      s[t][e + 1] = __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], c, nmc));
+      s[t][e] = __builtin_amdgcn_exp2f(s[t][e]);
+      s[t][e + 1] = __builtin_amdgcn_exp2f(s[t][e + 1]);
       r0 += s[t][e];
       r1 += s[t][e + 1];
     }
@@ -276,7 +280,7 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
 
 // Tiled forward: a workgroup owns 4 waves x QT x 32 query rows of one (batch entry, key head) and walks its share of the keys in chunks of 64.
 template <bool F16, int HD, int QT>
-__global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, HD <= 2 && QT == 1 ? 3 : 2) void xattn_fwd_kernel(const XArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * img_bytes<HD>() + KC * 4)];
   constexpr int BUF = 2 * img_bytes<HD>() + KC * 4;
   int bh, item;
@@ -327,24 +331,25 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
     if (row0 < a.R) {
       const bool biased = mask || (ch + 1) * KC > kend;
       f32x16 s[QT][2];
+      // (independent accumulators in turn: a product that waits for the one before it leaves the matrix unit idle; the first one starts at the
+      // inline constant 0 -- start values from LDS would cost every chunk the moves that only a chunk with hidden keys needs)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x16 init = splat(0.f);
-        if (biased) {
+      for (int ks = 0; ks < 2 * HD; ++ks)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const s16x8 kf = row_frag<HD>(K, t, ks);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt][t] = mma<F16>(kf, qf[qt][ks], ks ? s[qt][t] : splat(0.f));
+        }
+      if (biased) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float4 x = *reinterpret_cast<const float4*>(bs + t * 32 + 8 * g + 4 * hi);
-            init[4 * g] = x.x; init[4 * g + 1] = x.y; init[4 * g + 2] = x.z; init[4 * g + 3] = x.w;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) { s[qt][t][4 * g] += x.x; s[qt][t][4 * g + 1] += x.y; s[qt][t][4 * g + 2] += x.z; s[qt][t][4 * g + 3] += x.w; }
           }
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) s[qt][t] = init;
-#pragma unroll
-        for (int ks = 0; ks < 2 * HD; ++ks) {
-          const s16x8 kf = row_frag<HD>(K, t, ks);
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) s[qt][t] = mma<F16>(kf, qf[qt][ks], s[qt][t]);
-        }
       }
       s16x8 p[QT][4];
 #pragma unroll
@@ -354,9 +359,9 @@ __global__ __launch_bounds__(NT, 2) void xattn_fwd_kernel(const XArgs a) {
         for (int t = 0; t < 2; ++t) { p[qt][2 * t] = pack8<F16>(s[qt][t], 0); p[qt][2 * t + 1] = pack8<F16>(s[qt][t], 8); }
       }
 #pragma unroll
-      for (int db = 0; db < HD; ++db)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int db = 0; db < HD; ++db) {
           const s16x8 vf = tr_frag<HD>(V, db, k * 16);
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) o[qt][db] = mma<F16>(vf, p[qt][k], o[qt][db]);
@@ -540,7 +545,7 @@ __device__ __forceinline__ float row_start(float lse, float scale) { return lse 
 // SUMS (at most two chunks of keys): a pass of its own forms D = sum_k P dP from the fp32 products -- rowsum(dO * O) carries the rounding of O, most of
 // dS's error when a row's probabilities are spread over a few keys only.
 template <bool F16, int HD, bool SUMS>
-__global__ __launch_bounds__(NT, HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XArgs a) {
+__global__ __launch_bounds__(NT, HD <= 2 && !SUMS ? 3 : HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XArgs a) {
   constexpr int BUF = 2 * img_bytes<HD>() + KC * 4;
   __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
   int bh, item;
@@ -580,7 +585,7 @@ __global__ __launch_bounds__(NT, HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XAr
     for (int j = 0; j < 8; ++j) D = fmaf(to_f<F16>(df[ks][j]), to_f<F16>(of[j]), D);
   }
   D = half_sum(D);
-  const float s0 = row_start(lse, a.scale), c = a.scale * LOG2E;
+  const float c = a.scale * LOG2E, nl = live ? -lse * LOG2E : -INFINITY;   // P = exp2(c S + nl): 0 for a row without keys or past the end
   f32x16 dq[HD];
 #pragma unroll
   for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
@@ -600,7 +605,12 @@ __global__ __launch_bounds__(NT, HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XAr
       const bool biased = mask || (ch + 1) * KC > kend;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        f32x16 s = splat(s0), dp = splat(sums ? 0.f : -D);
+        f32x16 s, dp;
+#pragma unroll
+        for (int ks = 0; ks < 2 * HD; ++ks) {
+          s = mma<F16>(row_frag<HD>(K, t, ks), qf[ks], ks ? s : splat(0.f));
+          dp = mma<F16>(row_frag<HD>(V, t, ks), df[ks], ks ? dp : splat(0.f));
+        }
         if (biased) {
 #pragma unroll
           for (int gq = 0; gq < 4; ++gq) {
@@ -608,13 +618,11 @@ __global__ __launch_bounds__(NT, HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XAr
             s[4 * gq] += x.x; s[4 * gq + 1] += x.y; s[4 * gq + 2] += x.z; s[4 * gq + 3] += x.w;
           }
         }
+        const float off = SUMS && sums ? 0.f : D;
 #pragma unroll
-        for (int ks = 0; ks < 2 * HD; ++ks) {
-          s = mma<F16>(row_frag<HD>(K, t, ks), qf[ks], s);
-          dp = mma<F16>(row_frag<HD>(V, t, ks), df[ks], dp);
-        }
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, nl);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
+        for (int e = 0; e < 16; ++e) dp[e] = (dp[e] - off) * __builtin_amdgcn_exp2f(s[e]);
         if (SUMS && sums) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) Dx += dp[e];
@@ -622,10 +630,9 @@ __global__ __launch_bounds__(NT, HD <= 3 ? 2 : 1) void xattn_dq_kernel(const XAr
         }
         const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
-        for (int db = 0; db < HD; ++db) {
-          dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32), d0, dq[db]);
-          dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32 + 16), d1, dq[db]);
-        }
+        for (int db = 0; db < HD; ++db) dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32), d0, dq[db]);
+#pragma unroll
+        for (int db = 0; db < HD; ++db) dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32 + 16), d1, dq[db]);
       }
     }
     if (more) store(buf ^ 1);
@@ -704,6 +711,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
     if (any) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      if (t && ch * KC + 32 >= a.R) break;   // the last chunk's second tile holds no rows
       f32x16 s, dp;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -727,8 +735,11 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
 #pragma unroll
       for (int db = 0; db < HD; ++db) {
         dv[db] = mma<F16>(tr_frag<HD>(O, db, t * 32), p0, dv[db]);
-        dv[db] = mma<F16>(tr_frag<HD>(O, db, t * 32 + 16), p1, dv[db]);
         dk[db] = mma<F16>(tr_frag<HD>(Q, db, t * 32), d0, dk[db]);
+      }
+#pragma unroll
+      for (int db = 0; db < HD; ++db) {
+        dv[db] = mma<F16>(tr_frag<HD>(O, db, t * 32 + 16), p1, dv[db]);
         dk[db] = mma<F16>(tr_frag<HD>(Q, db, t * 32 + 16), d1, dk[db]);
       }
     }
@@ -950,16 +961,16 @@ __global__ __launch_bounds__(NT) void xattn_add_kernel(const float* __restrict__
 
 // ================================================================================================================== host
 constexpr int CUS = 256;
-struct Plan { bool few; int tiles, splits; };
+struct Plan { bool few; int tiles, per_wave, splits; };
 
 int round_up8(int64_t x) { return (int)((x + 7) / 8 * 8); }
 
 // Into how many pieces the contracted axis (`chunks` steps) of `blocks` workgroups is cut, so that the last round of workgroups over the card's
 // `slots` does not run half empty: the smallest estimated time of rounds * (steps + 2) * us_step, plus joining the fp32 partials (`mbytes` per
 // piece, written and read at ~4.5 TB/s, and a launch).  Estimates only rank the cuts; every cut gives a right result.
-int split_for(int64_t blocks, int chunks, int slots, double us_step, double mbytes) {
+int split_for(int64_t blocks, int chunks, int slots, double us_step, double mbytes, double& least) {
   int best = 1;
-  double least = 1e30;
+  least = 1e30;
   for (int s = 1; s <= 64 && s <= (chunks > 1 ? chunks / 2 : 1); ++s) {
     const double rounds = (double)((blocks * s + slots - 1) / slots), steps = (double)((chunks + s - 1) / s) + 2;
     const double t = rounds * steps * us_step + (s > 1 ? 4. + 2. * s * mbytes / 4.5 : 0.);
@@ -968,31 +979,36 @@ int split_for(int64_t blocks, int chunks, int slots, double us_step, double mbyt
   return best;
 }
 bool few_rows(int R) { return R <= 32; }
-// 32-row tiles per wave of the tiled forward: two share every K / V fragment read from LDS, where the registers hold them (head_dim <= 64) and 256-row
-// workgroups pad at most an eighth more rows than 128-row ones
-int row_tiles(int HD, int R) { return HD <= 2 && lt_cdiv(R, 256) * 16 <= lt_cdiv(R, 128) * 9 ? 2 : 1; }
-
-constexpr int SLOTS = 2 * CUS;     // workgroups of the tiled kernels that the card holds at a time
-// (us_step: a 64-token chunk of the tiled kernels at ~1 TFLOP/s a workgroup; a step of 4 x 32 keys of the few-row kernels)
+// Workgroups that a CU holds (registers) and the measured us of a 64-token chunk with that many on it, per 32 columns of head_dim:
+//   forward, one 32-row tile a wave     3 at head_dim <= 64: 1.15, 2 above: 0.63
+//   forward, two tiles a wave           2 at head_dim <= 64: 1.38 (they share every K / V fragment read from LDS: 15 % more rows per us when the card is full)
+//   dQ                                  3 at head_dim <= 64: 1.4,  2 above: 1.6;   dK / dV   2 at head_dim <= 64: 1.15, 1 above: 1.6
+// The few-row kernels walk 128 keys a step: 1.5 us (forward, 3 workgroups a CU), 2.5 us (backward, 2).
 Plan fwd_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int64_t bh = (int64_t)B * Hkv;
-  const int HD = lt_cdiv(dh, 32);
+  const int HD = lt_cdiv(dh, 32), chunks = lt_cdiv(Nk, KC);
   const double mb = 4e-6 * bh * R * dh;
-  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 128), 3 * CUS, 1.5, mb)};
-  const int rows = 128 * row_tiles(HD, R), tiles = lt_cdiv(R, rows);
-  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), SLOTS, 4e-6 * rows * KC * HD * 32, mb)};
+  double t1, t2;
+  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 3 * CUS, 1.5, mb, t1)};
+  const int n1 = lt_cdiv(R, 128), n2 = lt_cdiv(R, 256);
+  const int s1 = split_for(bh * n1, chunks, (HD <= 2 ? 3 : 2) * CUS, (HD <= 2 ? 1.15 : 0.63) * HD, mb, t1);
+  if (HD > 2) return {false, n1, 1, s1};
+  const int s2 = split_for(bh * n2, chunks, 2 * CUS, 1.38 * HD, mb, t2);
+  return t2 < t1 ? Plan{false, n2, 2, s2} : Plan{false, n1, 1, s1};
 }
 Plan dq_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int64_t bh = (int64_t)B * Hkv;
   const int HD = lt_cdiv(dh, 32), tiles = lt_cdiv(R, 128);
   const double mb = 4e-6 * bh * R * dh;
-  if (few_rows(R)) return {true, 1, split_for(bh, lt_cdiv(Nk, 128), SLOTS, 2.5, mb)};
-  return {false, tiles, split_for(bh * tiles, lt_cdiv(Nk, KC), SLOTS, 6e-6 * 128 * KC * HD * 32, mb)};
+  double t;
+  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 2 * CUS, 2.5, mb, t)};
+  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(Nk, KC), (HD <= 2 ? 3 : 2) * CUS, (HD <= 2 ? 1.4 : 1.6) * HD, mb, t)};
 }
 Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int HD = lt_cdiv(dh, 32), tiles = lt_cdiv(Nk, 128);
   const int64_t bh = (int64_t)B * Hkv;
-  return {false, tiles, split_for(bh * tiles, lt_cdiv(R, KC), SLOTS, 8e-6 * 128 * KC * HD * 32, 8e-6 * bh * Nk * dh)};
+  double t;
+  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(R, KC), (HD <= 2 ? 2 : 1) * CUS, (HD <= 2 ? 1.15 : 1.6) * HD, 8e-6 * bh * Nk * dh, t)};
 }
 int64_t fwd_floats(int B, int R, int Nk, int Hkv, int dh) {
   const Plan p = fwd_plan(B, R, Nk, Hkv, dh);
@@ -1047,11 +1063,11 @@ int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
     default: hipLaunchKernelGGL((KERNEL<F16, 4 __VA_ARGS__>), dim3(GRID), dim3(NT), 0, (hipStream_t)stream, a); break;   \
   }
 
-template <bool F16> void run_fwd(const XArgs& a, bool few, void* stream) {
+template <bool F16> void run_fwd(const XArgs& a, const Plan& p, void* stream) {
   const int64_t items = (int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits;
-  if (few) { XA_HD(xattn_fwd_few_kernel, (unsigned)items, F16) }
+  if (p.few) { XA_HD(xattn_fwd_few_kernel, (unsigned)items, F16) }
   else {
-    const int HD = lt_cdiv(a.dh, 32), qt = row_tiles(HD, a.R);
+    const int HD = lt_cdiv(a.dh, 32), qt = p.per_wave;
     if (HD == 1 && qt == 2) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 1, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
     else if (HD == 2 && qt == 2) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 2, 2>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
     else if (HD == 1) hipLaunchKernelGGL((xattn_fwd_kernel<F16, 1, 1>), dim3((unsigned)items), dim3(NT), 0, (hipStream_t)stream, a);
@@ -1119,8 +1135,8 @@ extern "C" int lt_cross_attention_fwd(const lt_cross_attention_desc* d, void* st
   LT_CHECK_ARG(need == 0 || (d->ws && aligned16(d->ws) && d->ws_floats >= need), "lt_cross_attention_fwd: a workspace of %lld floats is needed (got %lld)", (long long)need,
                (long long)(d->ws ? d->ws_floats : 0));
   LT_CHECK_ARG((int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits < (1ll << 31), "lt_cross_attention_fwd: too many workgroups");
-  if (d->dtype == LT_DT_F16) run_fwd<true>(a, p.few, stream);
-  else run_fwd<false>(a, p.few, stream);
+  if (d->dtype == LT_DT_F16) run_fwd<true>(a, p, stream);
+  else run_fwd<false>(a, p, stream);
   LT_CHECK_LAUNCH("lt_cross_attention_fwd");
 }
 
