@@ -66,38 +66,37 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// three maxima and a count over the workgroup, one pair of barriers
-__device__ __forceinline__ void block_max3_sum(float& x, float& y, float& z, int n, float* red, int& total) {
+// two maxima and a count over the workgroup, one pair of barriers
+__device__ __forceinline__ void block_max2_sum(float& x, float& y, int n, float* red, int& total) {
   x = wave_max(x);
   y = wave_max(y);
-  z = wave_max(z);
   float f = wave_sum((float)n);     // <= 1024: exact
   const int w = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
   float4* r = reinterpret_cast<float4*>(red);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) r[w] = make_float4(x, y, z, f);
+  if ((threadIdx.x & 63) == 0) r[w] = make_float4(x, y, f, 0.f);
   __syncthreads();
   float4 a = r[0];
-  for (int i = 1; i < nw; ++i) { const float4 b = r[i]; a = make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), a.w + b.w); }
-  x = a.x; y = a.y; z = a.z;
-  total = (int)a.w;
+  for (int i = 1; i < nw; ++i) { const float4 b = r[i]; a.x = fmaxf(a.x, b.x); a.y = fmaxf(a.y, b.y); a.z += b.z; }
+  x = a.x; y = a.y;
+  total = (int)a.z;
 }
-// three sums and, when asked, one in 64 bits
-__device__ __forceinline__ void block_sum3(float& x, float& y, float& z, double& p, float* red, double* redd, bool with_p) {
+// two sums, and two in 64 bits
+__device__ __forceinline__ void block_sum4(float& x, float& y, double& p, double& q, float* red, double* redd) {
   x = wave_sum(x);
   y = wave_sum(y);
-  z = wave_sum(z);
-  if (with_p) p = wave_sum_d(p);
+  p = wave_sum_d(p);
+  q = wave_sum_d(q);
   const int w = threadIdx.x >> 6, nw = (blockDim.x + 63) >> 6;
-  float4* r = reinterpret_cast<float4*>(red);
+  float2* r = reinterpret_cast<float2*>(red);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) { r[w] = make_float4(x, y, z, 0.f); redd[w] = p; }
+  if ((threadIdx.x & 63) == 0) { r[w] = make_float2(x, y); redd[2 * w] = p; redd[2 * w + 1] = q; }
   __syncthreads();
-  float4 a = r[0];
-  double q = redd[0];
-  for (int i = 1; i < nw; ++i) { const float4 b = r[i]; a.x += b.x; a.y += b.y; a.z += b.z; q += redd[i]; }
-  x = a.x; y = a.y; z = a.z;
-  p = q;
+  float2 a = r[0];
+  double b = redd[0], d = redd[1];
+  for (int i = 1; i < nw; ++i) { a.x += r[i].x; a.y += r[i].y; b += redd[2 * i]; d += redd[2 * i + 1]; }
+  x = a.x; y = a.y;
+  p = b; q = d;
 }
 __device__ __forceinline__ float teacher_value(const TopkArgs& a, int64_t row, int j) {
   const int64_t at = row * a.ldv + j;
@@ -114,16 +113,17 @@ __device__ __forceinline__ int teacher_class(const TopkArgs& a, int64_t row, int
 // Chunk i of thread t: E elements at (i * blockDim + t) * E.  The first NV chunks of a thread stay in registers, any further ones are read again in
 // every pass.  A workgroup walks rows blockIdx.x, + gridDim.x, ...: the next row's chunk is requested right behind the store of the chunk that held its
 // registers, its kept entries ahead of that.
-constexpr int EPT = 2;   // kept entries per thread that are requested ahead (all of them: k <= 1024, and workgroups that walk rows have 512 threads)
+constexpr int EPT = 1;   // kept entries per thread that are requested ahead (all of them up to k = 512: workgroups that walk rows have 512 threads)
 template <typename TS, typename TD, int E, int NV, int NTMAX>
 __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
-  extern __shared__ uint32_t dyn[];       // [ceil(max(K, NV * blockDim * E) / 32)] kept bits (set past K) | [k] class | [k] value, then probability | [k] student logit
+  extern __shared__ double dyn[];       // [k] exp(t) in 64 bits | [ceil(max(K, NV * blockDim * E) / 32)] kept bits (set past K) | [k] class | [k] teacher value | [k] student logit
   __shared__ __attribute__((aligned(16))) float red[64];
-  __shared__ double redd[16];
+  __shared__ double redd[32];
   __shared__ int twice;
   const int nt = blockDim.x, words = (max(a.K, NV * nt * E) + 31) >> 5;
-  uint32_t* bits = dyn;
-  int* cls = reinterpret_cast<int*>(dyn + words);
+  double* ex = dyn;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(dyn + a.k);
+  int* cls = reinterpret_cast<int*>(bits + words);
   float* val = reinterpret_cast<float*>(cls + a.k);
   float* zs = val + a.k;
   const int chunks = (a.K + E - 1) / E;
@@ -183,9 +183,9 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
       const int x = teacher_class(a, row, j);
       keep(j, x, teacher_value(a, row, j), x >= 0 ? getf(s[x]) : 0.f);
     }
-    if (more) entries(row + gridDim.x);
     __syncthreads();
     if (twice) {     // an index again in its row: its first entry counts
+#pragma unroll 1
       for (int j = threadIdx.x; j < a.k; j += nt) {
         const int x = teacher_class(a, row, j);
         bool again = false;
@@ -194,13 +194,27 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
       }
       __syncthreads();
     }
+    // ---- teacher probabilities, while the row itself is still on its way.  The loss is a difference of logarithms many times its size: its k terms and
+    // the logarithms it ends in are formed in 64 bits.
     float tmax = -INFINITY, zmax = -INFINITY;
     int mine = 0;
+#pragma unroll 1
     for (int j = threadIdx.x; j < a.k; j += nt)
       if (cls[j] >= 0) {
         ++mine;
         tmax = fmaxf(tmax, val[j]);
         zmax = fmaxf(zmax, zs[j]);
+      }
+    if (!a.t_lse) tmax = block_max(tmax, red);
+    const double tref = a.t_lse ? (double)a.t_lse[row] : (double)tmax * (double)a.inv_temp;
+    double psum = 0.0, cross = 0.0;
+#pragma unroll 1
+    for (int j = threadIdx.x; j < a.k; j += nt)
+      if (cls[j] >= 0) {
+        const double t = (double)val[j] * (double)a.inv_temp - tref, p = exp(t);
+        psum += p;
+        if (p > 0.0) cross += p * (t - (double)zs[j] * (double)a.inv_temp);
+        ex[j] = p;
       }
     // ---- the student's classes that are not kept: maximum, then the sum of exponentials against it.  A kept class becomes -inf here.
     auto hide = [&](int ch, PS& x) {
@@ -213,7 +227,7 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
     auto each = [&](auto&& f) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) f(v[i]);
-#pragma unroll 4
+#pragma unroll 2
       for (int ch = NV * nt + threadIdx.x; ch < chunks; ch += nt) {
         PS x = *reinterpret_cast<const PS*>(s + (int64_t)ch * E);
         hide(ch, x);
@@ -228,41 +242,25 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
       for (int e = 0; e < E; ++e) mrest = fmaxf(mrest, getf(x.v[e]));
     });
     int kept;
-    block_max3_sum(tmax, zmax, mrest, mine, red, kept);
+    block_max2_sum(zmax, mrest, mine, red, kept);
     const bool live = kept > 0 && w != 0.f && (a.t_lse || tmax > -INFINITY);   // otherwise nothing is known of this row, or nothing asked
     const float mr = mrest == -INFINITY ? 0.f : mrest, m = fmaxf(zmax, mrest);
-    float srest = 0.f, stop = 0.f, tsum = 0.f;
-    double psum = 0.0;
+    float srest = 0.f, stop = 0.f;
     // (differences first, then the scale: x c - m c would carry the rounding of m c into every term alike, and so into the loss)
     each([&](const PS& x) {
 #pragma unroll
       for (int e = 0; e < E; ++e) srest += __builtin_amdgcn_exp2f((getf(x.v[e]) - mr) * c);
     });
-    // ---- teacher probabilities and the kept classes' share of the student
+#pragma unroll 1
     for (int j = threadIdx.x; j < a.k; j += nt)
-      if (cls[j] >= 0) {
-        const float t = val[j];
-        if (a.t_lse) psum += exp((double)t * (double)a.inv_temp - (double)a.t_lse[row]);
-        else tsum += __expf((t - tmax) * a.inv_temp);
-        stop += __builtin_amdgcn_exp2f((zs[j] - m) * c);
-      }
-    block_sum3(srest, stop, tsum, psum, red, redd, a.t_lse != nullptr);
+      if (cls[j] >= 0) stop += __builtin_amdgcn_exp2f((zs[j] - m) * c);
+    block_sum4(srest, stop, psum, cross, red, redd);
     const float rest = a.t_lse && kept < a.K && psum < 1.0 ? (float)(1.0 - psum) : 0.f;
     const float frest = mrest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mrest - m) * c);
-    const float total = stop + srest * frest, lt = logf(total), ltsum = a.t_lse ? 0.f : logf(tsum);
+    const float total = stop + srest * frest, pmul = a.t_lse ? 1.f : (float)(1.0 / psum);
     const float g = w * a.inv_temp, gr = g * (frest / total - (srest > 0.f ? rest / srest : 0.f));
-    // ---- loss and gradient
-    float part = 0.f;
-    for (int j = threadIdx.x; j < a.k; j += nt)
-      if (cls[j] >= 0) {
-        const float z = (zs[j] - m) * a.inv_temp;
-        const float logp = a.t_lse ? (float)((double)val[j] * (double)a.inv_temp - (double)a.t_lse[row]) : (val[j] - tmax) * a.inv_temp - ltsum;
-        const float p = a.t_lse ? expf(logp) : __expf((val[j] - tmax) * a.inv_temp) / tsum;
-        if (p > 0.f) part += p * (logp - (z - lt));
-        val[j] = p;
-        zs[j] = __builtin_amdgcn_exp2f((zs[j] - m) * c) / total;
-      }
-    if (more) gather(sn);
+    // ---- gradient
+    if (more) { entries(row + gridDim.x); gather(sn); }
     const float cl = live ? c : 0.f, gl = live ? gr : 0.f, ml = live ? mr : 0.f;
     auto grad = [&](const PS& x) {
       PD o;
@@ -279,20 +277,24 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
       load(rn, i);
     }
     if (a.d) {
-#pragma unroll 4
+#pragma unroll 2
       for (int ch = NV * nt + threadIdx.x; ch < chunks; ch += nt) *reinterpret_cast<PD*>(d + (int64_t)ch * E) = grad(*reinterpret_cast<const PS*>(s + (int64_t)ch * E));
     }
-    part = block_sum(part, red);     // (its barriers also order the row's stores before the kept classes')
+    __syncthreads();     // the row's stores come before the kept classes'
     if (threadIdx.x == 0) {
-      if (rest > 0.f) part += rest * (logf(rest) - ((mr - m) * a.inv_temp + logf(srest) - lt));   // srest = 0: +inf
-      a.loss_rows[row] = live ? w * part : 0.f;
+      const double lt = log((double)total);
+      const double lq = (double)m * (double)a.inv_temp + lt;      // log sum exp of the student's row
+      double loss = a.t_lse ? cross + lq * psum : cross / psum - log(psum) + lq;
+      if (rest > 0.f) loss += (double)rest * (log((double)rest) - (((double)mr - (double)m) * (double)a.inv_temp + log((double)srest) - lt));   // srest = 0: +inf
+      a.loss_rows[row] = live ? (float)((double)w * loss) : 0.f;
       twice = 0;
     }
+#pragma unroll 1
     for (int j = threadIdx.x; j < a.k; j += nt) {
       const int x = cls[j];
       if (x < 0) continue;
       atomicAnd(&bits[x >> 5], ~(1u << (x & 31)));
-      if (a.d && live) d[x] = putf<TD>(g * (zs[j] - val[j]));
+      if (a.d && live) d[x] = putf<TD>(g * (__builtin_amdgcn_exp2f((zs[j] - m) * c) / total - (float)ex[j] * pmul));
     }
     __syncthreads();
   }
@@ -312,7 +314,7 @@ template <typename TS, typename TD, int E, int NV, int NTMAX> void go(const Topk
   int nt = 64;                        // the fewest waves whose registers hold the row
   while (nt < NTMAX && (int64_t)nt * NV < chunks) nt *= 2;
   const int bits = a.K > NV * nt * E ? a.K : NV * nt * E;
-  const size_t lds = ((size_t)((bits + 31) / 32) + 3 * (size_t)a.k) * 4;
+  const size_t lds = ((size_t)((bits + 31) / 32) + 5 * (size_t)a.k) * 4;
   hipLaunchKernelGGL((topk_kl_kernel<TS, TD, E, NV, NTMAX>), dim3(grid < a.rows ? grid : a.rows), dim3(nt), lds, st, a);
 }
 template <typename TS, typename TD> void dispatch(const TopkArgs& a, hipStream_t st) {
