@@ -58,6 +58,16 @@ template <bool F16> __device__ __forceinline__ s16x8 pack8(const f32x16& p, int 
                              pack2<F16>(p[off + 6], p[off + 7]));
   return __builtin_bit_cast(s16x8, u);
 }
+// a factor as two 16-bit parts, hi + lo: where memory bounds a kernel, a second product is free and the factor's rounding goes from 2^-9 to 2^-17 (f16: 2^-22)
+template <bool F16> __device__ __forceinline__ void split8(const f32x16& p, int off, s16x8& hi, s16x8& lo) {
+  hi = pack8<F16>(p, off);
+  f32x16 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = p[off + j] - to_f<F16>(hi[j]);
+#pragma unroll
+  for (int j = 8; j < 16; ++j) r[j] = 0.f;
+  lo = pack8<F16>(r, 0);
+}
 __device__ __forceinline__ f32x16 splat(float x) {
   f32x16 r;
 #pragma unroll
@@ -462,12 +472,17 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
     vf.store(img);
     load(t + 4);
     soft_step<HD, 1>(s, c, m, lsum, o);
-    const s16x8 p0 = pack8<F16>(s[0], 0), p1 = pack8<F16>(s[0], 8);
+    s16x8 p0, p1, q0, q1;
+    split8<F16>(s[0], 0, p0, q0);
+    split8<F16>(s[0], 8, p1, q1);
     wait_lds();
 #pragma unroll
     for (int db = 0; db < HD; ++db) {
-      o[db] = mma<F16>(tr_frag<HD>(img, db, 0), p0, o[db]);
-      o[db] = mma<F16>(tr_frag<HD>(img, db, 16), p1, o[db]);
+      const s16x8 v0 = tr_frag<HD>(img, db, 0), v1 = tr_frag<HD>(img, db, 16);
+      o[db] = mma<F16>(v0, p0, o[db]);
+      o[db] = mma<F16>(v0, q0, o[db]);
+      o[db] = mma<F16>(v1, p1, o[db]);
+      o[db] = mma<F16>(v1, q1, o[db]);
     }
     wait_lds();
   }
@@ -971,12 +986,17 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
     columns(kf, vf, all, -D, s, dp);
 #pragma unroll
     for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
-    s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
+    s16x8 d0, d1, e0, e1;
+    split8<F16>(dp, 0, d0, e0);
+    split8<F16>(dp, 8, d1, e1);
     wait_lds();
 #pragma unroll
     for (int db = 0; db < HD; ++db) {
-      dq[db] = mma<F16>(tr_frag<HD>(Kt, db, 0), d0, dq[db]);
-      dq[db] = mma<F16>(tr_frag<HD>(Kt, db, 16), d1, dq[db]);
+      const s16x8 k0 = tr_frag<HD>(Kt, db, 0), k1 = tr_frag<HD>(Kt, db, 16);
+      dq[db] = mma<F16>(k0, d0, dq[db]);
+      dq[db] = mma<F16>(k0, e0, dq[db]);
+      dq[db] = mma<F16>(k1, d1, dq[db]);
+      dq[db] = mma<F16>(k1, e1, dq[db]);
     }
     wait_lds();
     // lane -> key
@@ -998,21 +1018,28 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
       dp[e] *= p;
       s[e] = F16 ? p * P_UP : p;
     }
-    d0 = pack8<F16>(dp, 0);
-    d1 = pack8<F16>(dp, 8);
-    const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8);
+    split8<F16>(dp, 0, d0, e0);
+    split8<F16>(dp, 8, d1, e1);
     f32x16 acc[HD];
 #pragma unroll
     for (int db = 0; db < HD; ++db) {
-      acc[db] = mma<F16>(tr_frag<HD>(Q, db, 0), d0, splat(0.f));
-      acc[db] = mma<F16>(tr_frag<HD>(Q, db, 16), d1, acc[db]);
+      const s16x8 q0 = tr_frag<HD>(Q, db, 0), q1 = tr_frag<HD>(Q, db, 16);
+      acc[db] = mma<F16>(q0, d0, splat(0.f));
+      acc[db] = mma<F16>(q0, e0, acc[db]);
+      acc[db] = mma<F16>(q1, d1, acc[db]);
+      acc[db] = mma<F16>(q1, e1, acc[db]);
       if (!seen) acc[db] = splat(0.f);   // whatever dO holds
     }
     put_tile<F16, HD>(Kt, acc, a.scale, a.dh, [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(t * 32 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
+    split8<F16>(s, 0, d0, e0);
+    split8<F16>(s, 8, d1, e1);
 #pragma unroll
     for (int db = 0; db < HD; ++db) {
-      acc[db] = mma<F16>(tr_frag<HD>(O, db, 0), p0, splat(0.f));
-      acc[db] = mma<F16>(tr_frag<HD>(O, db, 16), p1, acc[db]);
+      const s16x8 o0 = tr_frag<HD>(O, db, 0), o1 = tr_frag<HD>(O, db, 16);
+      acc[db] = mma<F16>(o0, d0, splat(0.f));
+      acc[db] = mma<F16>(o0, e0, acc[db]);
+      acc[db] = mma<F16>(o1, d1, acc[db]);
+      acc[db] = mma<F16>(o1, e1, acc[db]);
       if (!seen) acc[db] = splat(0.f);
     }
     put_tile<F16, HD>(Kt, acc, F16 ? 1.f / P_UP : 1.f, a.dh,
