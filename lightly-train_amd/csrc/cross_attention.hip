@@ -12,7 +12,7 @@
 //   dQ        S^T, dP^T = V dO^T            ->  dQ^T = K^T dS^T
 //   dK / dV   S = Q K^T, dP = dO V^T (lane -> key)  ->  dV^T = dO^T P, dK^T = Q^T dS
 // One LDS image of a token chunk serves both kinds of operand: rows of d, and (ds_read_b64_tr_b16) columns whose contraction index is the token.
-// Keys that are not visible are staged as zeros (what the caller's padding holds is never multiplied) and their scores start at -inf.
+// Keys that are not visible are staged as zeros (what the caller's padding holds is never multiplied) and their scores are -inf.
 #include "lt_common.h"
 
 namespace {
@@ -358,7 +358,12 @@ __global__ __launch_bounds__(NT, HD <= 2 && QT == 1 ? 3 : 2) void xattn_fwd_kern
           for (int g = 0; g < 4; ++g) {
             const float4 x = *reinterpret_cast<const float4*>(bs + t * 32 + 8 * g + 4 * hi);
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) { s[qt][t][4 * g] += x.x; s[qt][t][4 * g + 1] += x.y; s[qt][t][4 * g + 2] += x.z; s[qt][t][4 * g + 3] += x.w; }
+            for (int qt = 0; qt < QT; ++qt) {   // (replaced, not added to: a query that holds NaN must not reach a row without keys)
+              s[qt][t][4 * g] = x.x < 0.f ? x.x : s[qt][t][4 * g];
+              s[qt][t][4 * g + 1] = x.y < 0.f ? x.y : s[qt][t][4 * g + 1];
+              s[qt][t][4 * g + 2] = x.z < 0.f ? x.z : s[qt][t][4 * g + 2];
+              s[qt][t][4 * g + 3] = x.w < 0.f ? x.w : s[qt][t][4 * g + 3];
+            }
           }
       }
       s16x8 p[QT][4];
@@ -464,11 +469,13 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
     if (seen != 0xffffffffu) {
       kf.hide(ok);
       vf.hide(ok);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[0][e] = (seen >> crow(e, hi)) & 1 ? 0.f : -INFINITY;
     }
 #pragma unroll
     for (int ks = 0; ks < 2 * HD; ++ks) s[0] = mma<F16>(kf.f[ks], qf[ks], s[0]);
+    if (seen != 0xffffffffu) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[0][e] = (seen >> crow(e, hi)) & 1 ? s[0][e] : -INFINITY;
+    }
     vf.store(img);
     load(t + 4);
     soft_step<HD, 1>(s, c, m, lsum, o);
