@@ -229,7 +229,9 @@ int lt_attention_bwd(const void* qkv, const void* out_bf16, const void* dout_bf1
  *   dtype      LT_DT_BF16 | LT_DT_F16 of q, k, v, out, dout, dq, dk, dv; scores, statistics and sums are fp32
  *   dh         8 .. 128, a multiple of 8, last dimension contiguous; s?? = element strides of (batch, token, head), multiples of 8, pointers
  *              16-byte aligned: views into a packed projection are read and written in place.  Stride 0 (a broadcast input) is allowed for
- *              inputs; outputs must not overlap each other or an input
+ *              inputs; outputs must not overlap each other or an input.  Token strides below 2^24 elements, Nk and Nq * H / Hkv below 2^24,
+ *              B * Hkv below 2^20; q k^T before the scale within +-1e30
+ *              (f16 gradients: P (dP - D) passes through f16, terms below 2^-24 are lost and above 65504 infinite -- scale the loss)
  *   key_lens   int32 [B] or NULL: keys >= key_lens[b] (clamped to 0 .. Nk) are not visible;  key_mask uint8 [B, Nk] or NULL: 0 = not visible.
  *              Keys that are not visible are not multiplied (their k, v may hold anything) and receive zero gradients; a row without any
  *              visible key gives out = 0, lse = -inf, dq = 0 and adds nothing to dk, dv
@@ -313,7 +315,8 @@ int lt_kl_fwd_bwd(const float* s_logits, const float* t_logits, int ld, float in
  * An index outside 0 .. K - 1 is a missing entry; of an index that comes again in its row the first entry counts; a row without entries, of weight 0
  * or (without t_lse) with all entries -inf gives loss 0 and gradient 0.
  *   s rows ld apart, LT_DT_*; dlogits rows ldd apart, the type of s, or bf16 for f32 s; t_val LT_DT_* rows ldv apart; t_idx int32 or (idx_is_64)
- *   int64 rows ldi apart; t_lse, row_weight f32 [rows] or NULL.  1 <= k <= 1024, k <= K <= 262144, inv_temp > 0 */
+ *   int64 rows ldi apart; t_lse, row_weight f32 [rows] or NULL.  dlogits must not overlap s.
+ *   1 <= k <= 1024, k <= K <= 262144, inv_temp > 0 */
 int lt_topk_kl_fwd_bwd(const void* s, int s_dtype, int64_t ld, const void* t_val, int val_dtype, int64_t ldv, const void* t_idx, int idx_is_64, int64_t ldi,
                        const float* t_lse, const float* row_weight, float inv_temp, float coef, float* loss_rows, float* loss, void* dlogits, int d_dtype,
                        int64_t ldd, int rows, int K, int k, void* stream);

@@ -1147,7 +1147,7 @@ Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
   if (R <= resident_rows(HD)) {   // no partials to join: cut the keys until the rounds are even; ~4 us to stage the rows, 4 tiles a step
     Plan p{true, 1, 1, 1};
     double least = 1e30;
-    for (int s = 1; s <= tiles; ++s) {
+    for (int s = 1; s <= tiles && (s == 1 || bh * s <= 16 * 2 * CUS); ++s) {   // (16 rounds: more cuts only stage the rows again)
       const double u = (double)((bh * s + 2 * CUS - 1) / (2 * CUS)) * (4. + 0.4 * HD * lt_cdiv(R, 32) * (double)((tiles + s - 1) / s));
       if (u < least) { least = u; p.splits = s; }
     }
@@ -1176,6 +1176,7 @@ bool strides_ok(const int64_t* s, int B, int N, int H) {
   return (B == 1 || (s[0] >= 0 && s[0] % 8 == 0)) && (N == 1 || (s[1] >= 0 && s[1] % 8 == 0 && s[1] < MAX_STEP)) && (H == 1 || (s[2] >= 0 && s[2] % 8 == 0));
 }
 Strides st3(const int64_t* s, int N) { return {s[0], N == 1 ? 128 : s[1], s[2]}; }   // (a single token has no step: any will do)
+constexpr int64_t MAX_GROUPS = 1 << 24;   // 256 threads each: a launch has fewer than 2^32
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
@@ -1186,11 +1187,11 @@ int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
   LT_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
   LT_CHECK_ARG((int64_t)d->Nq * (d->H / d->Hkv) < (1 << 24) && d->Nk < (1 << 24) && (int64_t)d->B * d->Hkv < (1 << 20), "%s: sizes out of range", who);
   const int G = d->H / d->Hkv;
-  if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->q && aligned16(d->q) && strides_ok(d->sq, d->B, d->Nq, d->H), "%s: q: 16-byte alignment of the pointer and of every stride", who);
+  if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->q && aligned16(d->q) && strides_ok(d->sq, d->B, d->Nq, d->H), "%s: q: 16-byte alignment of the pointer and of every stride, token stride below 2^24", who);
   if (d->Nk > 0 && d->B > 0)
     LT_CHECK_ARG(d->k && d->v && aligned16(d->k) && aligned16(d->v) && strides_ok(d->sk, d->B, d->Nk, d->Hkv) && strides_ok(d->sv, d->B, d->Nk, d->Hkv),
-                 "%s: k, v: 16-byte alignment of the pointers and of every stride", who);
-  if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->out && aligned16(d->out) && strides_ok(d->so, d->B, d->Nq, d->H), "%s: out: 16-byte alignment of the pointer and of every stride", who);
+                 "%s: k, v: 16-byte alignment of the pointers and of every stride, token strides below 2^24", who);
+  if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->out && aligned16(d->out) && strides_ok(d->so, d->B, d->Nq, d->H), "%s: out: 16-byte alignment of the pointer and of every stride, token stride below 2^24", who);
   a = XArgs{};
   a.q = (const uint16_t*)d->q; a.k = (const uint16_t*)d->k; a.v = (const uint16_t*)d->v;
   a.o = (const uint16_t*)d->out; a.out = (uint16_t*)d->out; a.lse = d->lse;
@@ -1254,11 +1255,11 @@ template <bool F16> void run_bwd(XArgs a, float* ws, void* stream) {
 }
 
 __global__ void xattn_zero_kernel(uint16_t* dst, Strides s, int64_t n, int N, int H, int d8) {
-  const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (i >= n) return;
-  const int c = (int)(i % d8), h = (int)(i / d8 % H);
-  const int64_t t = i / d8 / H;
-  *reinterpret_cast<uint4*>(dst + t / N * s.b + t % N * s.n + h * s.h + c * 8) = make_uint4(0, 0, 0, 0);
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
+    const int c = (int)(i % d8), h = (int)(i / d8 % H);
+    const int64_t t = i / d8 / H;
+    *reinterpret_cast<uint4*>(dst + t / N * s.b + t % N * s.n + h * s.h + c * 8) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 }  // namespace
@@ -1283,7 +1284,7 @@ extern "C" int lt_cross_attention_fwd(const lt_cross_attention_desc* d, void* st
   const int64_t need = fwd_floats(a.B, a.R, a.Nk, a.Hkv, a.dh);
   LT_CHECK_ARG(need == 0 || (d->ws && aligned16(d->ws) && d->ws_floats >= need), "lt_cross_attention_fwd: a workspace of %lld floats is needed (got %lld)", (long long)need,
                (long long)(d->ws ? d->ws_floats : 0));
-  LT_CHECK_ARG((int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits < (1ll << 31), "lt_cross_attention_fwd: too many workgroups");
+  LT_CHECK_ARG((int64_t)round_up8((int64_t)a.B * a.Hkv) * a.tiles * a.splits < MAX_GROUPS, "lt_cross_attention_fwd: too many workgroups");
   if (d->dtype == LT_DT_F16) run_fwd<true>(a, p, stream);
   else run_fwd<false>(a, p, stream);
   LT_CHECK_LAUNCH("lt_cross_attention_fwd");
@@ -1297,17 +1298,18 @@ extern "C" int lt_cross_attention_bwd(const lt_cross_attention_desc* d, void* st
   if (d->B == 0) return LT_OK;
   if (d->Nq > 0)
     LT_CHECK_ARG(d->lse && d->dout && d->dq && aligned16(d->dout) && aligned16(d->dq) && strides_ok(d->sdo, d->B, d->Nq, d->H) && strides_ok(d->sdq, d->B, d->Nq, d->H),
-                 "lt_cross_attention_bwd: lse, dout, dq: missing, or pointer or strides not 16-byte aligned");
+                 "lt_cross_attention_bwd: lse, dout, dq: missing, pointer or strides not 16-byte aligned, or a token stride of 2^24 or more");
   if (d->Nk > 0)
     LT_CHECK_ARG(d->dk && d->dv && aligned16(d->dk) && aligned16(d->dv) && strides_ok(d->sdk, d->B, d->Nk, d->Hkv) && strides_ok(d->sdv, d->B, d->Nk, d->Hkv),
-                 "lt_cross_attention_bwd: dk, dv: missing, or pointer or strides not 16-byte aligned");
+                 "lt_cross_attention_bwd: dk, dv: missing, pointer or strides not 16-byte aligned, or a token stride of 2^24 or more");
   a.dout = (const uint16_t*)d->dout; a.dq = (uint16_t*)d->dq; a.dk = (uint16_t*)d->dk; a.dv = (uint16_t*)d->dv;
   a.sdo = st3(d->sdo, d->Nq); a.sdq = st3(d->sdq, d->Nq); a.sdk = st3(d->sdk, d->Nk); a.sdv = st3(d->sdv, d->Nk);
   if (d->Nq == 0) {   // no queries: the keys' gradients are zero
     if (d->Nk > 0) {
       const int64_t n = (int64_t)a.B * a.Nk * a.Hkv * (a.dh / 8);
-      hipLaunchKernelGGL(xattn_zero_kernel, dim3((unsigned)lt_cdiv(n, NT)), dim3(NT), 0, (hipStream_t)stream, a.dk, a.sdk, n, a.Nk, a.Hkv, a.dh / 8);
-      hipLaunchKernelGGL(xattn_zero_kernel, dim3((unsigned)lt_cdiv(n, NT)), dim3(NT), 0, (hipStream_t)stream, a.dv, a.sdv, n, a.Nk, a.Hkv, a.dh / 8);
+      const unsigned grid = (unsigned)(n < 64 * CUS * NT ? lt_cdiv(n, NT) : 64 * CUS);
+      hipLaunchKernelGGL(xattn_zero_kernel, dim3(grid), dim3(NT), 0, (hipStream_t)stream, a.dk, a.sdk, n, a.Nk, a.Hkv, a.dh / 8);
+      hipLaunchKernelGGL(xattn_zero_kernel, dim3(grid), dim3(NT), 0, (hipStream_t)stream, a.dv, a.sdv, n, a.Nk, a.Hkv, a.dh / 8);
     }
     LT_CHECK_LAUNCH("lt_cross_attention_bwd");
   }
@@ -1316,7 +1318,7 @@ extern "C" int lt_cross_attention_bwd(const lt_cross_attention_desc* d, void* st
                (long long)(d->ws ? d->ws_floats : 0));
   const int64_t bh8 = round_up8((int64_t)a.B * a.Hkv);
   const Plan p1 = dq_plan(a.B, a.R, a.Nk, a.Hkv, a.dh), p2 = dkdv_plan(a.B, a.R, a.Nk, a.Hkv, a.dh);
-  LT_CHECK_ARG(bh8 * p1.tiles * p1.splits < (1ll << 31) && bh8 * p2.tiles * p2.splits < (1ll << 31), "lt_cross_attention_bwd: too many workgroups");
+  LT_CHECK_ARG(bh8 * p1.tiles * p1.splits < MAX_GROUPS && bh8 * p2.tiles * p2.splits < MAX_GROUPS, "lt_cross_attention_bwd: too many workgroups");
   if (d->dtype == LT_DT_F16) run_bwd<true>(a, d->ws, stream);
   else run_bwd<false>(a, d->ws, stream);
   LT_CHECK_LAUNCH("lt_cross_attention_bwd");

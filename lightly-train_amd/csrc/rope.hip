@@ -133,7 +133,7 @@ extern "C" int lt_rope_axes(const lt_rope_axes_desc* d, void* stream) {
   a.sx = st3(d->sx); a.so = st3(d->so); a.sx2 = st3(d->sx2); a.so2 = st3(d->so2);
   a.tokens = (int64_t)d->B * d->N; a.pos_b = d->pos_per_batch ? d->N - d->prefix : 0;
   a.N = d->N; a.H = d->H; a.H2 = d->H2; a.dh = d->dh; a.prefix = d->prefix; a.axes = d->axes; a.pos_float = d->pos_float; a.inverse = d->inverse;
-  LT_CHECK_ARG(a.tokens / (NT / (d->dh >> 1)) < (1ll << 31) - 1, "lt_rope_axes: too many tokens");
+  LT_CHECK_ARG(a.tokens / (NT / (d->dh >> 1)) < (1ll << 24) - 1, "lt_rope_axes: too many tokens");
   hipStream_t st = (hipStream_t)stream;
   if (d->dtype == LT_DT_F32) launch<float, 4>(a, d->interleaved, st);
   else if (d->dtype == LT_DT_BF16) { if (d->dh % 16 == 0) launch<bf_t, 8>(a, d->interleaved, st); else launch<bf_t, 4>(a, d->interleaved, st); }

@@ -495,7 +495,7 @@ def topk_kl_fwd_bwd(s: Tensor, t_val: Tensor, t_idx: Tensor, inv_temp: float, co
     """KL divergence from a teacher known by k top logits a row (t_val bf16 / f16 / f32, t_idx int32 / int64, [rows, k]) to softmax(s * inv_temp), s [rows, K]
     bf16 / f16 / f32: loss_rows f32 [rows] (overwritten), loss f32 [1] += their sum, dlogits [rows, K] (the type of s, or bf16 for f32 s).  t_lse f32 [rows]:
     the log-sum-exp of the teacher's whole row * inv_temp; with it the classes not kept are one bucket, without it the kept logits are renormalised.  Index < 0
-    (or >= K): no entry; of a repeated index the first entry counts.  Row r is weighted by coef * row_weight[r] (lt_topk_kl_fwd_bwd)."""
+    (or >= K): no entry; of a repeated index the first entry counts.  dlogits must not overlap s.  Row r is weighted by coef * row_weight[r] (lt_topk_kl_fwd_bwd)."""
     who = "topk_kl_fwd_bwd"
     if s.dim() != 2 or t_val.dim() != 2 or s.dtype not in _DT:
         raise ValueError(f"{who}: s [rows, K] of bfloat16, float16 or float32 and t_val [rows, k], got {s.dtype} {tuple(s.shape)} and {tuple(t_val.shape)}")
@@ -781,8 +781,9 @@ def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Optio
                         key_mask: Optional[Tensor] = None, ws: Optional[Tensor] = None) -> None:
     """out = softmax(scale * q k^T) v for queries q [B, Nq, H, dh] against another sequence's k, v [B, Nk, Hkv, dh] (bf16 or f16, strided views
     allowed, H a multiple of Hkv); lse f32 [B, H, Nq] (needed by the backward) or None.  key_lens int32 [B], key_mask bool / uint8 [B, Nk]: which keys
-    are visible; a row without one gives out = 0, lse = -inf.  ws: f32 scratch of `cross_attention_fwd_ws_floats` elements, allocated
-    here when None; calls that may run at the same time need their own (lt_cross_attention_fwd)."""
+    are visible; a row without one gives out = 0, lse = -inf.  Token strides below 2^24 elements; out must not overlap an input.
+    ws: f32 scratch of `cross_attention_fwd_ws_floats` elements, allocated here when None; calls that may run at the same time need their own
+    (lt_cross_attention_fwd)."""
     _xattn("cross_attention_fwd", "lt_cross_attention_fwd", cross_attention_fwd_ws_floats, q, k, v, out, lse, scale, key_lens, key_mask, ws)
 
 
