@@ -1100,15 +1100,18 @@ struct Plan { bool few; int tiles, per_wave, splits; };
 
 int round_up8(int64_t x) { return (int)((x + 7) / 8 * 8); }
 
-// Into how many pieces the contracted axis (`chunks` steps) of `blocks` workgroups is cut, so that the last round of workgroups over the card's
-// `slots` does not run half empty: the smallest estimated time of rounds * (steps + 2) * us_step, plus joining the fp32 partials (`mbytes` per
-// piece, written and read at ~4.5 TB/s, and a launch).  Estimates only rank the cuts; every cut gives a right result.
-int split_for(int64_t blocks, int chunks, int slots, double us_step, double mbytes, double& least) {
+// Into how many pieces the contracted axis (`chunks` steps) of `blocks` workgroups is cut, `per_cu` of which a CU holds: the smallest estimated time of
+// rounds * (steps + 2) * us_step, plus joining the fp32 partials (`mbytes` per piece: 3.3 MB 4.2 us for 2, 5.5 for 4, 7.9 for 8; 13 MB 8.9 for 2, 15 for 5).  A last round that
+// puts n workgroups on a CU costs 1/3 + 2/3 n / per_cu of a full one (measured at head_dim 64: 2.05, 2.8, 3.7 us a chunk with 1, 2, 3 of them): 128
+// workgroups over 16 chunks take 30 us uncut, 20.5 + 4 (join) in 2, 17 + 5 in 4 and 17.4 + 6.3 in 6 pieces.  Estimates only rank the cuts; every cut
+// gives a right result.
+int split_for(int64_t blocks, int chunks, int per_cu, double us_step, double mbytes, double& least) {
   int best = 1;
   least = 1e30;
   for (int s = 1; s <= 64 && s <= (chunks > 1 ? chunks / 2 : 1); ++s) {
-    const double rounds = (double)((blocks * s + slots - 1) / slots), steps = (double)((chunks + s - 1) / s) + 2;
-    const double t = rounds * steps * us_step + (s > 1 ? 4. + 2. * s * mbytes / 4.5 : 0.);
+    const int64_t full = blocks * s / (per_cu * CUS), rest = blocks * s - full * per_cu * CUS;
+    const double rounds = (double)full + (rest ? 1. / 3. + 2. / 3. * (double)((rest + CUS - 1) / CUS) / per_cu : 0.), steps = (double)((chunks + s - 1) / s) + 2;
+    const double t = rounds * steps * us_step + (s > 1 ? 3. + 0.2 * s * mbytes : 0.);
     if (t < least) { least = t; best = s; }
   }
   return best;
@@ -1124,11 +1127,11 @@ Plan fwd_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int HD = lt_cdiv(dh, 32), chunks = lt_cdiv(Nk, KC);
   const double mb = 4e-6 * bh * R * dh;
   double t1, t2;
-  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 3 * CUS, 1.5, mb, t1)};
+  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 3, 1.5, mb, t1)};
   const int n1 = lt_cdiv(R, 128), n2 = lt_cdiv(R, 256);
-  const int s1 = split_for(bh * n1, chunks, (HD <= 2 ? 3 : 2) * CUS, (HD <= 2 ? 1.15 : 0.63) * HD, mb, t1);
+  const int s1 = split_for(bh * n1, chunks, HD <= 2 ? 3 : 2, (HD <= 2 ? 1.15 : 0.63) * HD, mb, t1);
   if (HD > 2) return {false, n1, 1, s1};
-  const int s2 = split_for(bh * n2, chunks, 2 * CUS, 1.38 * HD, mb, t2);
+  const int s2 = split_for(bh * n2, chunks, 2, 1.38 * HD, mb, t2);
   return t2 < t1 ? Plan{false, n2, 2, s2} : Plan{false, n1, 1, s1};
 }
 Plan dq_plan(int B, int R, int Nk, int Hkv, int dh) {
@@ -1136,8 +1139,8 @@ Plan dq_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int HD = lt_cdiv(dh, 32), tiles = lt_cdiv(R, 128);
   const double mb = 4e-6 * bh * R * dh;
   double t;
-  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 2 * CUS, 2.5, mb, t)};
-  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(Nk, KC), (HD <= 2 ? 3 : 2) * CUS, (HD <= 2 ? 1.4 : 1.6) * HD, mb, t)};
+  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 2, 2.5, mb, t)};
+  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(Nk, KC), HD <= 2 ? 3 : 2, (HD <= 2 ? 1.4 : 1.6) * HD, mb, t)};
 }
 int resident_rows(int HD) { return HD == 1 ? rows_resident<1>() : HD == 2 ? rows_resident<2>() : HD == 3 ? rows_resident<3>() : rows_resident<4>(); }
 Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
@@ -1153,7 +1156,7 @@ Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
     }
     return p;
   }
-  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(R, KC), (HD <= 2 ? 2 : 1) * CUS, (HD <= 2 ? 1.15 : 1.6) * HD, 8e-6 * bh * Nk * dh, t)};
+  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(R, KC), HD <= 2 ? 2 : 1, (HD <= 2 ? 1.15 : 1.6) * HD, 8e-6 * bh * Nk * dh, t)};
 }
 int64_t fwd_floats(int B, int R, int Nk, int Hkv, int dh) {
   const Plan p = fwd_plan(B, R, Nk, Hkv, dh);
