@@ -13,6 +13,10 @@
 //   dK / dV   S = Q K^T, dP = dO V^T (lane -> key)  ->  dV^T = dO^T P, dK^T = Q^T dS
 // One LDS image of a token chunk serves both kinds of operand: rows of d, and (ds_read_b64_tr_b16) columns whose contraction index is the token.
 // Keys that are not visible are staged as zeros (what the caller's padding holds is never multiplied) and their scores are -inf.
+//
+// Roundings to 16 bits: the tiled kernels round P and dS once on their way into the second product, which makes a result's error sqrt(2) of its own rounding
+// (measured 1.1 - 1.4 for O, 1.4 for dV, 1.4 - 1.5 for dK and 1.4 - 1.55 for dQ, to which D from the rounded O adds); both halves of dS would cost dQ
+// a third more matrix work.  The few-row kernels, which memory bounds, multiply both halves (measured 1.00, dQ <= 1.06).
 #include "lt_common.h"
 
 namespace {
@@ -289,6 +293,9 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
 }
 
 // Tiled forward: a workgroup owns 4 waves x QT x 32 query rows of one (batch entry, key head) and walks its share of the keys in chunks of 64.
+// No unit is saturated: counted, the matrix unit is busy 22 % (head_dim 128: 40 %) of the cycles, the vector unit by estimate 45 - 50 %, 22 - 37 % of
+// the waves' time is waiting; wave priorities around the products and the compiler's interleaving options moved nothing.  1569 x 2 rows against 6273 keys x 16 heads of 64, masked, 160 - 168 us
+// = 480 - 510 TFLOP/s over the visible and hidden keys; 3136 rows x 25 088 keys x 8 of 128, 380 - 426 us = 760 - 850 TFLOP/s (a large matrix product reaches 1195).
 template <bool F16, int HD, int QT>
 __global__ __launch_bounds__(NT, HD <= 2 && QT == 1 ? 3 : 2) void xattn_fwd_kernel(const XArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[2 * (2 * img_bytes<HD>() + KC * 4)];
@@ -406,7 +413,8 @@ __global__ __launch_bounds__(NT, HD <= 2 && QT == 1 ? 3 : 2) void xattn_fwd_kern
 
 // Few rows (R <= 32: pooling by one query, one new token): the waves share the one row tile and split the KEYS.  K fragments are rows and come
 // straight from memory, V passes through a wave-private image; the next tile's loads are in flight while a tile is computed.  Bound by reading
-// K / V: the padded matrix work of a 32-key tile (8 HD MFMAs) hides under its 8 KiB * HD / 2 of loads.
+// K / V: the padded matrix work of a 32-key tile (12 HD MFMAs) hides under its 8 KiB * HD / 2 of loads.
+// 768 heads x 1370 keys of 64: 50 - 54 us (270 MB; 54 us at the 5.03 TB/s of a copy; repeated on the same tensors, some of which the cache still holds); 384 x 785: 17 us.
 template <int HD> struct KeyTile {
   s16x8 f[2 * HD];
   __device__ __forceinline__ void load(const uint16_t* base, int64_t sn, int key, bool ok, int dh) {
@@ -563,7 +571,8 @@ __global__ __launch_bounds__(NT) void xattn_join_kernel(const XArgs a) {
 // A row without keys has lse = -inf: it starts at -inf like a row past the end, and every P is 0.
 __device__ __forceinline__ float row_start(float lse, float scale) { return lse == -INFINITY ? -INFINITY : -lse / scale; }
 
-// dQ: a workgroup owns 128 query rows and walks its share of the keys; D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
+// dQ: a workgroup owns 128 query rows and walks its share of the keys (196 rows x 1370 keys x 384 heads of 64: 67 us = 590 TFLOP/s; 64 columns and one row tile a
+// wave leave three waves to a SIMD -- four spill: 76 -> 165 us, and two row tiles a wave leave two: 74 -> 89 us); D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
 // SUMS (at most two chunks of keys): a pass of its own forms D = sum_k P dP from the fp32 products -- rowsum(dO * O) carries the rounding of O, most of
 // dS's error when a row's probabilities are spread over a few keys only.
 template <bool F16, int HD, bool SUMS>
@@ -671,7 +680,8 @@ __global__ __launch_bounds__(NT, HD <= 2 && !SUMS ? 3 : HD <= 3 ? 2 : 1) void xa
   });
 }
 
-// dK / dV: a wave owns 32 keys (K, V fragments and both accumulators in registers), the query rows pass through LDS in chunks of 64.
+// dK / dV: a wave owns 32 keys (K, V fragments and both accumulators in registers), the query rows pass through LDS in chunks of 64
+// (3138 rows x 6273 keys x 16 heads of 64, masked, the matrix unit busy 31 % of it, waves waiting 44 %: 235 - 247 us = 650 - 685 TFLOP/s, hidden keys counted).
 template <bool F16, int HD>
 __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const XArgs a) {
   constexpr int BUF = 2 * img_bytes<HD>() + 2 * KC * 4;
@@ -890,7 +900,8 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_rows_kernel(co
 
 // Few rows (R <= 32): every key tile meets the one row tile once, so dK / dV of the tile are complete at once and all three gradients take ONE pass
 // over K / V.  Each wave owns key tiles; S is formed in both orientations (lane -> key for dK / dV, lane -> query for dQ): the second set of
-// products costs less than turning dS through LDS, and the pass is bound by memory.
+// products costs less than turning dS through LDS, and the pass is bound by memory (384 heads x 785 keys of 64, 155 MB: 38 us = 4.0 TB/s; without the second halves of the
+// rounded factors 34 us).
 template <bool F16, int HD>
 __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(const XArgs a) {
   constexpr int IMG = 32 * HD * 64, OST = HD * 32 + 4;

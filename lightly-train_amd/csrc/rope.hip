@@ -5,6 +5,8 @@
 // Bound by memory (every element read and written once).  A workgroup takes T tokens; the dh / 2 angles of a token are formed ONCE, in 64 bits
 // (position * frequency in fp32 is off by 0.06 rad at position 10^6), reduced to a quarter turn there, and their sines and cosines stay in
 // registers while a thread walks the heads of q and k: T = 256 / (dh / 2) tokens, one angle per thread, 8 (4) head lanes.
+// 154 MB of bf16 q and k of video tokens: 26 us warm (5.9 TB/s, part of it from the cache; 36 us a call with fresh tensors); 538 MB of fp32: 104 us = 5.2 TB/s,
+// the rate of a copy.
 #include "lt_common.h"
 
 namespace {
