@@ -1,7 +1,7 @@
 """Builds liblt_amd.so (the C-ABI HIP library) in-tree with hipcc for gfx950.
 
 hipcc cross-compiles without a GPU, so this also runs in the CPU-only build container.
-Objects are cached by source mtime; the .so is git-ignored but travels with gpurun snapshots.
+Objects are cached by source mtime; the .so is git-ignored and lies in the tree.
 """
 from __future__ import annotations
 
