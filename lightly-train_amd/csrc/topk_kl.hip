@@ -3,7 +3,9 @@
 //   kept classes j: without t_lse p_j = softmax over the kept t_j / T; with t_lse (the teacher's log-sum-exp over all K at that temperature)
 //   p_j = exp(t_j / T - t_lse), and everything else is one bucket, p_rest = max(0, 1 - sum p_j) against q_rest = sum of q over the classes not kept.
 //   loss = w (sum_j p_j (log p_j - log q_j) + p_rest (log p_rest - log q_rest)),   w = coef * row_weight
-//   dlogits = w / T * { q_j - p_j  kept;  q_i (1 - p_rest / q_rest)  others }
+//   dlogits = w / T * { m q_j - p_j  kept;  q_i (m - p_rest / q_rest)  others },   m = sum p_j + p_rest
+// m is 1 wherever there is a bucket (p_rest = 1 - sum p_j) and for renormalised values.  Kept probabilities whose sum passes 1 (values stored in 16 bits next to a
+// 32-bit t_lse: up to 1.04 for a sure teacher), or rows of which every class is kept, have no bucket: there m = sum p_j, or the gradient were not the loss's.
 // Bound by memory: the row is read once and its gradient written once.  The registers of a workgroup of 512 threads hold a row of up to 65 536 fp32 (32
 // pieces of 16 bytes a thread) between the three passes over it (maximum, sum of exponentials, gradient); what does not fit is read again, through the
 // caches (a sixteenth of the row costs ~10 us at 2048 x 65 536).  One workgroup to a CU walks the rows and requests each piece of the next row behind
@@ -260,7 +262,7 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
     const float rest = a.t_lse && kept < a.K && psum < 1.0 ? (float)(1.0 - psum) : 0.f;
     const float frest = mrest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mrest - m) * c);
     const float total = stop + srest * frest, pmul = a.t_lse ? 1.f : (float)(1.0 / psum);
-    const float g = w * a.inv_temp, gr = g * (frest / total - (srest > 0.f ? rest / srest : 0.f));
+    const float g = w * a.inv_temp, mass = a.t_lse && rest == 0.f ? (float)psum : 1.f, gr = g * (frest / total * mass - (srest > 0.f ? rest / srest : 0.f));
     // ---- gradient
     if (more) { entries(row + gridDim.x); gather(sn); }
     const float cl = live ? c : 0.f, gl = live ? gr : 0.f, ml = live ? mr : 0.f;
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
       const int x = cls[j];
       if (x < 0) continue;
       atomicAnd(&bits[x >> 5], ~(1u << (x & 31)));
-      if (a.d && live) d[x] = putf<TD>(g * (__builtin_amdgcn_exp2f((zs[j] - m) * c) / total - (float)ex[j] * pmul));
+      if (a.d && live) d[x] = putf<TD>(g * (__builtin_amdgcn_exp2f((zs[j] - m) * c) / total * mass - (float)ex[j] * pmul));
     }
     __syncthreads();
   }

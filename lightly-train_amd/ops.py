@@ -494,7 +494,8 @@ def topk_kl_fwd_bwd(s: Tensor, t_val: Tensor, t_idx: Tensor, inv_temp: float, co
                     t_lse: Optional[Tensor] = None, row_weight: Optional[Tensor] = None, loss: Optional[Tensor] = None) -> None:
     """KL divergence from a teacher known by k top logits a row (t_val bf16 / f16 / f32, t_idx int32 / int64, [rows, k]) to softmax(s * inv_temp), s [rows, K]
     bf16 / f16 / f32: loss_rows f32 [rows] (overwritten), loss f32 [1] += their sum, dlogits [rows, K] (the type of s, or bf16 for f32 s).  t_lse f32 [rows]:
-    the log-sum-exp of the teacher's whole row * inv_temp; with it the classes not kept are one bucket, without it the kept logits are renormalised.  Index < 0
+    the log-sum-exp of the teacher's whole row * inv_temp; with it the classes not kept are one bucket, without it the kept logits are renormalised.  Values whose
+    probabilities sum past 1 beside t_lse (16-bit storage) are taken as they are: no bucket is left, and the gradient is that of the returned loss.  Index < 0
     (or >= K): no entry; of a repeated index the first entry counts.  dlogits must not overlap s.  Row r is weighted by coef * row_weight[r] (lt_topk_kl_fwd_bwd)."""
     who = "topk_kl_fwd_bwd"
     if s.dim() != 2 or t_val.dim() != 2 or s.dtype not in _DT:
