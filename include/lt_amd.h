@@ -314,7 +314,7 @@ int lt_kl_fwd_bwd(const float* s_logits, const float* t_logits, int ld, float in
  *   dlogits[r]   = w * inv_temp * (m q_j - p_j on kept classes, q_i * (m - p_rest / q_rest) elsewhere), m = sum_j p_j + p_rest       (dlogits may be NULL)
  * (m is 1 except where the kept probabilities pass 1, as values stored in 16 bits may beside a 32-bit t_lse, or where every class is kept: m = sum_j p_j)
  * An index outside 0 .. K - 1 is a missing entry; of an index that comes again in its row the first entry counts; a row without entries, of weight 0
- * or (without t_lse) with all entries -inf gives loss 0 and gradient 0.
+ * or (without t_lse) with all entries -inf gives loss 0 and gradient 0.  A NaN among a row's entries or logits shows in its loss and gradient.
  *   s rows ld apart, LT_DT_*; dlogits rows ldd apart, the type of s, or bf16 for f32 s; t_val LT_DT_* rows ldv apart; t_idx int32 or (idx_is_64)
  *   int64 rows ldi apart; t_lse, row_weight f32 [rows] or NULL.  dlogits must not overlap s.
  *   1 <= k <= 1024, k <= K <= 262144, inv_temp > 0 */

@@ -206,7 +206,7 @@ __global__ __launch_bounds__(NTMAX) void topk_kl_kernel(const TopkArgs a) {
     for (int j = threadIdx.x; j < a.k; j += nt)
       if (cls[j] >= 0) {
         ++mine;
-        tmax = fmaxf(tmax, val[j]);
+        tmax = fmaxf(tmax, val[j] == val[j] ? val[j] : INFINITY);     // (fmaxf drops NaN: a row that knows nothing else would pass for one without entries)
         zmax = fmaxf(zmax, zs[j]);
       }
     if (!a.t_lse) tmax = block_max(tmax, red);
