@@ -15,7 +15,7 @@
 // Keys that are not visible are staged as zeros (what the caller's padding holds is never multiplied) and their scores are -inf.
 //
 // Roundings to 16 bits: the tiled kernels round P and dS once on their way into the second product, which makes a result's error sqrt(2) of its own rounding
-// (measured 1.1 - 1.4 for O, 1.4 for dV, 1.4 - 1.5 for dK and 1.4 - 1.55 for dQ, to which D from the rounded O adds); both halves of dS would cost dQ
+// (measured 1.1 - 1.4 for O, 1.4 for dV, 1.4 - 1.5 for dK and 1.4 - 1.57 for dQ, to which D from the rounded O adds); both halves of dS would cost dQ
 // a third more matrix work.  The few-row kernels, which memory bounds, multiply both halves (measured 1.00, dQ <= 1.06).
 #include "lt_common.h"
 
@@ -31,6 +31,11 @@ constexpr float M_NONE = -1e30f;   // running maximum before the first visible k
 constexpr int NT = 256;            // threads per workgroup, four waves
 constexpr int KC = 64;             // tokens per LDS chunk of the tiled kernels
 constexpr float P_UP = 4096.f;     // f16 probabilities of the backward are kept times 2^12: 1 / Nk of a long cache would be subnormal
+// The forward's probabilities are kept <= 2^GROW (soft_step).  f16: times 2^11 and GROW 4, so <= 2^15 and rounded at 2^-36 of a row's largest at worst: below that the long
+// tail behind a dominant key was lost from P V (25 % of its weight at e^-18) while its sum of exponentials counted it.  All 2^24 keys that a call may have
+// lose 2^-12 of the result there, half of its own rounding.  The sums carry the factor too: it cancels in O and is divided out of the sum in lse.
+template <bool F16> constexpr float P_GROW = F16 ? 4.f : 8.f;
+template <bool F16> constexpr float P_LOG2 = F16 ? 11.f : 0.f;
 
 struct Strides { int64_t b, n, h; };
 struct XArgs {
@@ -62,7 +67,8 @@ template <bool F16> __device__ __forceinline__ s16x8 pack8(const f32x16& p, int 
                              pack2<F16>(p[off + 6], p[off + 7]));
   return __builtin_bit_cast(s16x8, u);
 }
-// a factor as two 16-bit parts, hi + lo: where memory bounds a kernel, a second product is free and the factor's rounding goes from 2^-9 to 2^-17 (f16: 2^-22)
+// a factor as two 16-bit parts, hi + lo: where memory bounds a kernel, a second product is free and the factor's rounding goes from 2^-9 to 2^-17 (f16: 2^-22, as
+// far as lo is a normal number: from 2^-3 on)
 template <bool F16> __device__ __forceinline__ void split8(const f32x16& p, int off, s16x8& hi, s16x8& lo) {
   hi = pack8<F16>(p, off);
   f32x16 r;
@@ -255,16 +261,16 @@ template <int HD> __device__ __forceinline__ void put_partial(float* dst, const 
 
 // ================================================================================================================== forward
 // One online-softmax step of one 32-query tile over NK 32-key tiles of raw scores s (base 2, reference m in raw-score units that moves only when a
-// row's maximum passes it by more than 8 octaves: probabilities stay <= 2^8, exact in fp32 and bf16 / f16 safe).  lsum is per lane (the two halves
-// of a row are added once, at the end).
-template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[NK], float c, float& m, float& lsum, f32x16 (&o)[HD]) {
+// row's maximum passes it by more than P_GROW octaves: probabilities stay <= 2^8, exact in fp32 and bf16 safe; f16: <= 2^4, times 2^11).  lsum is per lane (the
+// two halves of a row are added once, at the end).
+template <bool F16, int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[NK], float c, float& m, float& lsum, f32x16 (&o)[HD]) {
   float mx = s[0][0];
 #pragma unroll
   for (int t = 0; t < NK; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
   mx = half_max(mx);
-  const bool grow = (mx - m) * c > 8.f;
+  const bool grow = (mx - m) * c > P_GROW<F16>;
   if (__builtin_amdgcn_ballot_w64(grow) != 0) {
     const float mn = grow ? mx : m, alpha = __builtin_amdgcn_exp2f((m - mn) * c);
     lsum *= alpha;
@@ -274,7 +280,7 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
   }
-  const float nmc = -m * c;
+  const float nmc = fmaf(-m, c, P_LOG2<F16>);
   float r0 = 0.f, r1 = 0.f;
 #pragma unroll
   for (int t = 0; t < NK; ++t)
@@ -290,6 +296,11 @@ template <int HD, int NK> __device__ __forceinline__ void soft_step(f32x16 (&s)[
       r1 += s[t][e + 1];
     }
   lsum += r0 + r1;
+}
+
+// ln of a row's sum of exponentials
+template <bool F16> __device__ __forceinline__ float row_lse(float m, float lsum, float scale) {
+  return lsum != 0.f ? m * scale + __logf(F16 ? lsum * 0x1p-11f : lsum) : -INFINITY;
 }
 
 // Tiled forward: a workgroup owns 4 waves x QT x 32 query rows of one (batch entry, key head) and walks its share of the keys in chunks of 64.
@@ -376,7 +387,7 @@ __global__ __launch_bounds__(NT, HD <= 2 && QT == 1 ? 3 : 2) void xattn_fwd_kern
       s16x8 p[QT][4];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        soft_step<HD, 2>(s[qt], c, m[qt], lsum[qt], o[qt]);
+        soft_step<F16, HD, 2>(s[qt], c, m[qt], lsum[qt], o[qt]);
 #pragma unroll
         for (int t = 0; t < 2; ++t) { p[qt][2 * t] = pack8<F16>(s[qt][t], 0); p[qt][2 * t + 1] = pack8<F16>(s[qt][t], 8); }
       }
@@ -406,7 +417,7 @@ __global__ __launch_bounds__(NT, HD <= 2 && QT == 1 ? 3 : 2) void xattn_fwd_kern
         const int rr = row0 + t * 32 + x, g = rr / a.Nq, n = rr - g * a.Nq;
         return rr < a.R ? a.out + b * a.so.b + n * a.so.n + (int64_t)(hk * a.G + g) * a.so.h : nullptr;
       });
-      if (hi == 0 && a.lse && r < a.R) a.lse[((int64_t)b * a.H + hk * a.G) * a.Nq + r] = ls != 0.f ? m[t] * a.scale + __logf(ls) : -INFINITY;   // (rows of a group lie one after the other)
+      if (hi == 0 && a.lse && r < a.R) a.lse[((int64_t)b * a.H + hk * a.G) * a.Nq + r] = row_lse<F16>(m[t], ls, a.scale);   // (rows of a group lie one after the other)
     }
   }
 }
@@ -486,7 +497,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
     }
     vf.store(img);
     load(t + 4);
-    soft_step<HD, 1>(s, c, m, lsum, o);
+    soft_step<F16, HD, 1>(s, c, m, lsum, o);
     s16x8 p0, p1, q0, q1;
     split8<F16>(s[0], 0, p0, q0);
     split8<F16>(s[0], 8, p1, q1);
@@ -534,7 +545,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 3 : 2) void xattn_fwd_few_kernel(cons
       const float inv = ls != 0.f ? 1.f / ls : 0.f;
       *reinterpret_cast<uint2*>(a.out + b * a.so.b + nn * a.so.n + h * a.so.h + d) =
           make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
-      if (d == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + nn] = ls != 0.f ? mm * a.scale + __logf(ls) : -INFINITY;
+      if (d == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + nn] = row_lse<F16>(mm, ls, a.scale);
     }
   }
 }
@@ -563,7 +574,7 @@ __global__ __launch_bounds__(NT) void xattn_join_kernel(const XArgs a) {
   }
   const float inv = ls != 0.f ? 1.f / ls : 0.f;
   *reinterpret_cast<uint2*>(a.out + b * a.so.b + n * a.so.n + h * a.so.h + d) = make_uint2(pack2<F16>(acc.x * inv, acc.y * inv), pack2<F16>(acc.z * inv, acc.w * inv));
-  if (d == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + n] = ls != 0.f ? mm * a.scale + __logf(ls) : -INFINITY;
+  if (d == 0 && a.lse) a.lse[((int64_t)b * a.H + h) * a.Nq + n] = row_lse<F16>(mm, ls, a.scale);
 }
 
 // ================================================================================================================== backward
