@@ -231,8 +231,7 @@ int lt_attention_bwd(const void* qkv, const void* out_bf16, const void* dout_bf1
  *              16-byte aligned: views into a packed projection are read and written in place.  Stride 0 (a broadcast input) is allowed for
  *              inputs; outputs must not overlap each other or an input.  Token strides below 2^24 elements, Nk and Nq * H / Hkv below 2^24,
  *              B * Hkv below 2^20; q k^T before the scale within +-1e30
- *              (f16: P is rounded at 2^-36 of a row's largest at worst)
- *              (f16 gradients: P (dP - D) passes through f16, terms below 2^-24 are lost and above 65504 infinite -- scale the loss)
+ *              (f16: P is rounded at 2^-36 of a row's largest at worst, P (dP - D) at 2^-36 of its row's or key's largest, whatever the upstream scale)
  *   key_lens   int32 [B] or NULL: keys >= key_lens[b] (clamped to 0 .. Nk) are not visible;  key_mask uint8 [B, Nk] or NULL: 0 = not visible.
  *              Keys that are not visible are not multiplied (their k, v may hold anything) and receive zero gradients; a row without any
  *              visible key gives out = 0, lse = -inf, dq = 0 and adds nothing to dk, dv

@@ -582,6 +582,45 @@ __global__ __launch_bounds__(NT) void xattn_join_kernel(const XArgs a) {
 // A row without keys has lse = -inf: it starts at -inf like a row past the end, and every P is 0.
 __device__ __forceinline__ float row_start(float lse, float scale) { return lse == -INFINITY ? -INFINITY : -lse / scale; }
 
+// f16 dS = P (dP - D) carries P's 1 / Nk and the size of the upstream gradient: unscaled it lost bits from 2^-14 on, long before the gradients are that small (1.6 % of dQ
+// at 784 x 25 088 and an upstream scale of 1e-3), and was infinite past 65504 where they are not.  It is rounded times 2^up instead, up its column's (dQ: a query
+// row's, dK: a key's) own: from 40, where dS from 2^-54 on is a normal number, up goes down whenever the column's largest passes 2^15 -- to 2^11 .. 2^12, so that it
+// seldom does again -- and the accumulators with it, as under a running maximum.  A column's dS is rounded at 2^-36 of its largest at worst.  2^up comes out
+// with the store.
+constexpr int DS_UP = 40;
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+__device__ __forceinline__ int octaves_down(float mx) { return mx > 32768.f ? max(__builtin_amdgcn_frexp_expf(mx) - 12, 0) : 0; }   // (infinities: 0)
+__device__ __forceinline__ float column_max(const f32x16& x) {   // |x| over the two lanes that hold a column
+  float mx = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(x[e]));
+  return half_max(mx);
+}
+// s, dp: S - lse / scale, dP - D -> P times 2^12 = P_UP and dS times 2^up
+__device__ __forceinline__ void scaled_factors(f32x16& s, f32x16& dp, float c, int up) {
+  const float f = pow2(up - 12);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, 12.f);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    s[e] = __builtin_amdgcn_exp2f(s[e]);
+    dp[e] *= s[e] * f;
+  }
+}
+template <int HD> __device__ __forceinline__ void bring_down(f32x16& ds, int& up, f32x16 (&acc)[HD]) {
+  const float mx = column_max(ds);
+  if (__builtin_amdgcn_ballot_w64(mx > 32768.f) == 0) return;
+  const int n = octaves_down(mx);
+  const float f = pow2(-n);
+  up -= n;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) ds[e] *= f;
+#pragma unroll
+  for (int db = 0; db < HD; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[db][e] *= f;
+}
+
 // dQ: a workgroup owns 128 query rows and walks its share of the keys (196 rows x 1370 keys x 384 heads of 64: 67 us = 590 TFLOP/s; 64 columns and one row tile a
 // wave leave three waves to a SIMD -- four spill: 76 -> 165 us, and two row tiles a wave leave two: 74 -> 89 us); D = rowsum(dO * O) of its rows is formed here and left for the dK / dV kernel.
 // SUMS (at most two chunks of keys): a pass of its own forms D = sum_k P dP from the fp32 products -- rowsum(dO * O) carries the rounding of O, most of
@@ -635,6 +674,7 @@ __global__ __launch_bounds__(NT, HD <= 2 && !SUMS ? 3 : HD <= 3 ? 2 : 1) void xa
   __syncthreads();
   const int first = SUMS ? c_hi - c_lo : 0, all = first + c_hi - c_lo;
   float Dx = 0.f;
+  int up = F16 ? DS_UP : 0;
   for (int it = 0; it < all; ++it) {
     const bool more = it + 1 < all, sums = SUMS && it < first;
     const int ch = c_lo + (sums || !SUMS ? it : it - first), buf = it & 1;
@@ -660,9 +700,9 @@ __global__ __launch_bounds__(NT, HD <= 2 && !SUMS ? 3 : HD <= 3 ? 2 : 1) void xa
             s[4 * gq] += x.x; s[4 * gq + 1] += x.y; s[4 * gq + 2] += x.z; s[4 * gq + 3] += x.w;
           }
         }
-        const float off = SUMS && sums ? 0.f : D;
+        const float off = SUMS && sums ? 0.f : D, nu = F16 && !(SUMS && sums) ? nl + (float)up : nl;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, nl);
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, nu);
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = (dp[e] - off) * __builtin_amdgcn_exp2f(s[e]);
         if (SUMS && sums) {
@@ -670,6 +710,7 @@ __global__ __launch_bounds__(NT, HD <= 2 && !SUMS ? 3 : HD <= 3 ? 2 : 1) void xa
           for (int e = 0; e < 16; ++e) Dx += dp[e];
           continue;
         }
+        if constexpr (F16) bring_down<HD>(dp, up, dq);
         const s16x8 d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
         for (int db = 0; db < HD; ++db) dq[db] = mma<F16>(tr_frag<HD>(K, db, t * 32), d0, dq[db]);
@@ -681,11 +722,12 @@ __global__ __launch_bounds__(NT, HD <= 2 && !SUMS ? 3 : HD <= 3 ? 2 : 1) void xa
     __syncthreads();
   }
   if (split == 0 && hi == 0 && r < a.R) a.delta[(int64_t)bh * a.R + r] = D;
+  const float mul = F16 ? __builtin_amdgcn_ldexpf(a.scale, -up) : a.scale;
   if (a.splits > 1) {
-    if (r < a.R) put_partial<HD>(a.ws + ((int64_t)split * a.B * a.Hkv * a.R + (int64_t)bh * a.R + r) * a.dh, dq, a.scale, a.dh);
+    if (r < a.R) put_partial<HD>(a.ws + ((int64_t)split * a.B * a.Hkv * a.R + (int64_t)bh * a.R + r) * a.dh, dq, mul, a.dh);
     return;
   }
-  put_tile<F16, HD>(smem + wave * (32 * HD * 64), dq, a.scale, a.dh, [&](int x) -> uint16_t* {
+  put_tile<F16, HD>(smem + wave * (32 * HD * 64), dq, mul, a.dh, [&](int x) -> uint16_t* {
     const int rr = row0 + x, gg = rr / a.Nq, nn = rr - gg * a.Nq;
     return rr < a.R ? a.dq + b * a.sdq.b + nn * a.sdq.n + (int64_t)(hk * a.G + gg) * a.sdq.h : nullptr;
   });
@@ -741,6 +783,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
 #pragma unroll
   for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
   const float c = a.scale * LOG2E;
+  int up = F16 ? DS_UP : 0;
   const bool any = __builtin_amdgcn_ballot_w64(seen) != 0;
   if (c_lo < c_hi) store(0);
   __syncthreads();
@@ -768,11 +811,15 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
         s = mma<F16>(row_frag<HD>(Q, t, ks), kf.f[ks], s);
         dp = mma<F16>(row_frag<HD>(O, t, ks), vf.f[ks], dp);
       }
+      if constexpr (F16) {
+        scaled_factors(s, dp, c, up);
+        bring_down<HD>(dp, up, dk);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[e] * c);
-        dp[e] *= p;
-        s[e] = F16 ? p * P_UP : p;
+        for (int e = 0; e < 16; ++e) {
+          s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+          dp[e] *= s[e];
+        }
       }
       const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8), d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
@@ -794,17 +841,17 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_kernel(const X
 #pragma unroll
     for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
   }
-  const float vmul = F16 ? 1.f / P_UP : 1.f;
+  const float vmul = F16 ? 1.f / P_UP : 1.f, kmul = F16 ? __builtin_amdgcn_ldexpf(a.scale, -up) : a.scale;
   if (a.splits > 1) {
     if (key >= a.Nk) return;
     const int64_t keys = (int64_t)a.B * a.Hkv * a.Nk, at = split * keys + (int64_t)bh * a.Nk + key;
-    put_partial<HD>(a.ws + at * a.dh, dk, a.scale, a.dh);
+    put_partial<HD>(a.ws + at * a.dh, dk, kmul, a.dh);
     put_partial<HD>(a.ws + (a.splits * keys + at) * a.dh, dv, vmul, a.dh);
     return;
   }
   const int key0 = (tile * 4 + wave) * 32;
   char* img = smem + wave * (32 * HD * 64);
-  put_tile<F16, HD>(img, dk, a.scale, a.dh, [&](int x) -> uint16_t* { return key0 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(key0 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
+  put_tile<F16, HD>(img, dk, kmul, a.dh, [&](int x) -> uint16_t* { return key0 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(key0 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
   put_tile<F16, HD>(img, dv, vmul, a.dh, [&](int x) -> uint16_t* { return key0 + x < a.Nk ? a.dv + b * a.sdv.b + (int64_t)(key0 + x) * a.sdv.n + hk * a.sdv.h : nullptr; });
 }
 
@@ -865,6 +912,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_rows_kernel(co
     f32x16 dk[HD], dv[HD];
 #pragma unroll
     for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
+    int up = F16 ? DS_UP : 0;
     for (int x = 0; x < (all ? rt : 0); ++x) {
       f32x16 s, dp;
 #pragma unroll
@@ -879,13 +927,17 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_rows_kernel(co
         s = mma<F16>(row_frag<HD>(Q, x, ks), kf.f[ks], s);
         dp = mma<F16>(row_frag<HD>(O, x, ks), vf.f[ks], dp);
       }
+      if constexpr (F16) {   // (a hidden key's column is replaced by zeros below)
+        scaled_factors(s, dp, c, up);
+        bring_down<HD>(dp, up, dk);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] *= c;
+        for (int e = 0; e < 16; ++e) s[e] *= c;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[e]);   // (a hidden key's column is replaced by zeros below)
-        dp[e] *= p;
-        s[e] = F16 ? p * P_UP : p;
+        for (int e = 0; e < 16; ++e) {
+          s[e] = __builtin_amdgcn_exp2f(s[e]);
+          dp[e] *= s[e];
+        }
       }
       const s16x8 p0 = pack8<F16>(s, 0), p1 = pack8<F16>(s, 8), d0 = pack8<F16>(dp, 0), d1 = pack8<F16>(dp, 8);
 #pragma unroll
@@ -903,7 +955,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_dkdv_rows_kernel(co
 #pragma unroll
       for (int db = 0; db < HD; ++db) { dk[db] = splat(0.f); dv[db] = splat(0.f); }
     }
-    put_tile<F16, HD>(img, dk, a.scale, a.dh, [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(t * 32 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
+    put_tile<F16, HD>(img, dk, F16 ? __builtin_amdgcn_ldexpf(a.scale, -up) : a.scale, a.dh, [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(t * 32 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
     put_tile<F16, HD>(img, dv, F16 ? 1.f / P_UP : 1.f, a.dh,
                       [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dv + b * a.sdv.b + (int64_t)(t * 32 + x) * a.sdv.n + hk * a.sdv.h : nullptr; });
   }
@@ -967,6 +1019,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
   }
   D = half_sum(D);
   f32x16 dq[HD];
+  int up = F16 ? DS_UP : 0;
 #pragma unroll
   for (int db = 0; db < HD; ++db) dq[db] = splat(0.f);
   __syncthreads();
@@ -1014,7 +1067,8 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
     f32x16 s, dp;
     columns(kf, vf, all, -D, s, dp);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(s[e] * c);
+    for (int e = 0; e < 16; ++e) dp[e] *= __builtin_amdgcn_exp2f(F16 ? fmaf(s[e], c, (float)up) : s[e] * c);
+    if constexpr (F16) bring_down<HD>(dp, up, dq);
     s16x8 d0, d1, e0, e1;
     split8<F16>(dp, 0, d0, e0);
     split8<F16>(dp, 8, d1, e1);
@@ -1041,11 +1095,20 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
       s = mma<F16>(row_frag<HD>(Q, 0, ks), kf.f[ks], s);
       dp = mma<F16>(row_frag<HD>(O, 0, ks), vf.f[ks], dp);
     }
+    float kmul = a.scale;   // (a hidden key's column is replaced by zeros below)
+    if constexpr (F16) {   // every product of a key is here: its largest to 2^11 .. 2^12
+      scaled_factors(s, dp, c, 12);
+      const int n = min(12 - __builtin_amdgcn_frexp_expf(column_max(dp)), 100);   // (2^n stays finite)
+      const float f = pow2(n);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float p = __builtin_amdgcn_exp2f(s[e] * c);   // (a hidden key's column is replaced by zeros below)
-      dp[e] *= p;
-      s[e] = F16 ? p * P_UP : p;
+      for (int e = 0; e < 16; ++e) dp[e] *= f;
+      kmul = __builtin_amdgcn_ldexpf(a.scale, -12 - n);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(s[e] * c);
+        dp[e] *= s[e];
+      }
     }
     split8<F16>(dp, 0, d0, e0);
     split8<F16>(dp, 8, d1, e1);
@@ -1059,7 +1122,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
       acc[db] = mma<F16>(q1, e1, acc[db]);
       if (!seen) acc[db] = splat(0.f);   // whatever dO holds
     }
-    put_tile<F16, HD>(Kt, acc, a.scale, a.dh, [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(t * 32 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
+    put_tile<F16, HD>(Kt, acc, kmul, a.dh, [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dk + b * a.sdk.b + (int64_t)(t * 32 + x) * a.sdk.n + hk * a.sdk.h : nullptr; });
     split8<F16>(s, 0, d0, e0);
     split8<F16>(s, 8, d1, e1);
 #pragma unroll
@@ -1075,7 +1138,7 @@ __global__ __launch_bounds__(NT, HD <= 2 ? 2 : 1) void xattn_bwd_few_kernel(cons
                       [&](int x) -> uint16_t* { return t * 32 + x < a.Nk ? a.dv + b * a.sdv.b + (int64_t)(t * 32 + x) * a.sdv.n + hk * a.sdv.h : nullptr; });
   }
   __syncthreads();   // images -> the waves' partial dQ rows
-  if (r < a.R) put_partial<HD>(reinterpret_cast<float*>(smem) + (wave * 32 + r) * OST, dq, a.scale, HD * 32);
+  if (r < a.R) put_partial<HD>(reinterpret_cast<float*>(smem) + (wave * 32 + r) * OST, dq, F16 ? __builtin_amdgcn_ldexpf(a.scale, -up) : a.scale, HD * 32);
   __syncthreads();
   const float* part = reinterpret_cast<const float*>(smem);
   const int d4n = a.dh >> 2;
