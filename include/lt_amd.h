@@ -247,7 +247,7 @@ typedef struct lt_cross_attention_desc {
   const void* dout; void* dq; void* dk; void* dv;   /* backward only */
   int64_t sq[3], sk[3], sv[3], so[3], sdo[3], sdq[3], sdk[3], sdv[3];
   int B, Nq, Nk, H, Hkv, dh, dtype;
-  float scale;                    /* > 0 */
+  float scale;                    /* 2^-100 .. 2^100 */
   float* ws; int64_t ws_floats;
 } lt_cross_attention_desc;
 int64_t lt_cross_attention_fwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh);

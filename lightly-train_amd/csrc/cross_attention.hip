@@ -280,7 +280,7 @@ template <bool F16, int HD, int NK> __device__ __forceinline__ void soft_step(f3
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
   }
-  const float nmc = fmaf(-m, c, P_LOG2<F16>);
+  const float nmc = fminf(fmaf(-m, c, P_LOG2<F16>), 3e38f);   // (finite, also for M_NONE at a large scale: a hidden key's -inf stays -inf)
   float r0 = 0.f, r1 = 0.f;
 #pragma unroll
   for (int t = 0; t < NK; ++t)
@@ -1264,6 +1264,7 @@ bool strides_ok(const int64_t* s, int B, int N, int H) {
   return (B == 1 || (s[0] >= 0 && s[0] % 8 == 0)) && (N == 1 || (s[1] >= 0 && s[1] % 8 == 0 && s[1] < MAX_STEP)) && (H == 1 || (s[2] >= 0 && s[2] % 8 == 0));
 }
 Strides st3(const int64_t* s, int N) { return {s[0], N == 1 ? 128 : s[1], s[2]}; }   // (a single token has no step: any will do)
+constexpr float MIN_SCALE = 0x1p-100f, MAX_SCALE = 0x1p100f;   // lse / scale and scale * log2(e) have to be finite
 constexpr int64_t MAX_GROUPS = 1 << 24;   // 256 threads each: a launch has fewer than 2^32
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -1272,7 +1273,7 @@ int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
                d->Nq, d->Nk, d->H, d->Hkv);
   LT_CHECK_ARG(d->dh >= 8 && d->dh <= 128 && d->dh % 8 == 0, "%s: head_dim must be a multiple of 8 from 8 to 128 (got %d)", who, d->dh);
   LT_CHECK_ARG(d->dtype == LT_DT_BF16 || d->dtype == LT_DT_F16, "%s: dtype must be LT_DT_BF16 or LT_DT_F16", who);
-  LT_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", who);
+  LT_CHECK_ARG(d->scale >= MIN_SCALE && d->scale <= MAX_SCALE, "%s: scale must lie between 2^-100 and 2^100", who);
   LT_CHECK_ARG((int64_t)d->Nq * (d->H / d->Hkv) < (1 << 24) && d->Nk < (1 << 24) && (int64_t)d->B * d->Hkv < (1 << 20), "%s: sizes out of range", who);
   const int G = d->H / d->Hkv;
   if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->q && aligned16(d->q) && strides_ok(d->sq, d->B, d->Nq, d->H), "%s: q: 16-byte alignment of the pointer and of every stride, token stride below 2^24", who);

@@ -729,6 +729,7 @@ def cross_attention_bwd_ws_floats(B: int, Nq: int, Nk: int, H: int, Hkv: int, dh
 
 
 _XATTN = struct.Struct("@11P24q7ifPq")      # lt_cross_attention_desc (_lib.CrossAttentionDesc)
+_MIN_SCALE, _MAX_SCALE = 2.0 ** -100, 2.0 ** 100
 _KEY_MASK, _KEY_LENS = (torch.bool, torch.uint8), (torch.int32,)
 
 
@@ -746,8 +747,8 @@ def _xattn(who: str, fn: str, ws_floats: Any, q: Tensor, k: Tensor, v: Tensor, o
         raise ValueError(f"{who}: the query heads ({H}) must be a multiple of the key heads ({Hkv})")
     if dh % 8 or not 8 <= dh <= 128:
         raise ValueError(f"{who}: head_dim must be a multiple of 8 from 8 to 128, got {dh}")
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"{who}: scale must be positive and finite, got {scale}")
+    if not _MIN_SCALE <= scale <= _MAX_SCALE:
+        raise ValueError(f"{who}: scale must lie between 2^-100 and 2^100, got {scale}")
     dev = _device()
     sk = (B, Nk, Hkv, dh)
     tq, tk, tv = _strided(q, sq, dt, dev, who + ".q"), _strided(k, sk, dt, dev, who + ".k"), _strided(v, sk, dt, dev, who + ".v")

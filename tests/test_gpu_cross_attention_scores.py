@@ -48,3 +48,23 @@ def test_both_directions_of_peaked_rows(Nq, Nk, H, Hkv, dh, dt, spread):
     k = torch.where(seen[:, :, None, None], (k.float() + ramp).to(dt), k)
     o = _run(q, k, v, do, scale, lens, km)
     _check(o, _exact(q, k, v, do, seen, scale), q, k, dt, scale, seen)
+
+
+@pytest.mark.parametrize("Nq,Nk", [(2, 400), (100, 400)])
+@pytest.mark.parametrize("scale", [2.0 ** -90, 1e-9, 1e9, 2.0 ** 60])
+def test_scales_far_from_one_with_hidden_keys_first(Nq, Nk, scale):
+    """The scores are of size 1; the first 200 keys are hidden (the running maximum still holds no key after three chunks)."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    h = (1.0 / (8 * scale)) ** 0.5                                        # q and k take half of 1 / scale each
+    q, k, v, do = (rnd(1, Nq, 2, 64) * h).to(BF), (rnd(1, Nk, 2, 64) * h).to(BF), rnd(1, Nk, 2, 64).to(BF), rnd(1, Nq, 2, 64).to(BF)
+    km = torch.ones(1, Nk, dtype=torch.bool, device="cuda")
+    km[:, :200] = False
+    o = _run(q, k, v, do, scale, None, km)
+    r = _exact(q, k, v, do, km, scale)
+    for n, size in (("out", 1.0), ("dq", scale * h), ("dk", scale * h), ("dv", 1.0)):      # compared at the size that the scale leaves them
+        r[n], o[n] = r[n] / size, o[n].double() / size
+    assert ((o["lse"].double() - r["lse"]).abs() < 1e-5).all()
+    for n in ("out", "dq", "dk", "dv"):      # four roundings of P / dS, out in D and the result, norm-wise
+        assert torch.isfinite(o[n]).all(), n
+        assert float((o[n] - r[n]).norm()) <= 4 * 2.0 ** -8 * float(r[n].norm()), n
