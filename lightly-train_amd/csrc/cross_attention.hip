@@ -1268,13 +1268,16 @@ constexpr float MIN_SCALE = 0x1p-100f, MAX_SCALE = 0x1p100f;   // lse / scale an
 constexpr int64_t MAX_GROUPS = 1 << 24;   // 256 threads each: a launch has fewer than 2^32
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// (what the plans may be asked about: their 32-bit row counts hold it)
+bool in_range(int B, int Nq, int Nk, int H, int Hkv) { return (int64_t)Nq * (H / Hkv) < (1 << 24) && Nk < (1 << 24) && (int64_t)B * Hkv < (1 << 20); }
+
 int fill(const lt_cross_attention_desc* d, XArgs& a, const char* who) {
   LT_CHECK_ARG(d->B >= 0 && d->Nq >= 0 && d->Nk >= 0 && d->H > 0 && d->Hkv > 0 && d->H % d->Hkv == 0, "%s: bad sizes (B %d, Nq %d, Nk %d, H %d, Hkv %d)", who, d->B,
                d->Nq, d->Nk, d->H, d->Hkv);
   LT_CHECK_ARG(d->dh >= 8 && d->dh <= 128 && d->dh % 8 == 0, "%s: head_dim must be a multiple of 8 from 8 to 128 (got %d)", who, d->dh);
   LT_CHECK_ARG(d->dtype == LT_DT_BF16 || d->dtype == LT_DT_F16, "%s: dtype must be LT_DT_BF16 or LT_DT_F16", who);
   LT_CHECK_ARG(d->scale >= MIN_SCALE && d->scale <= MAX_SCALE, "%s: scale must lie between 2^-100 and 2^100", who);
-  LT_CHECK_ARG((int64_t)d->Nq * (d->H / d->Hkv) < (1 << 24) && d->Nk < (1 << 24) && (int64_t)d->B * d->Hkv < (1 << 20), "%s: sizes out of range", who);
+  LT_CHECK_ARG(in_range(d->B, d->Nq, d->Nk, d->H, d->Hkv), "%s: sizes out of range", who);
   const int G = d->H / d->Hkv;
   if (d->Nq > 0 && d->B > 0) LT_CHECK_ARG(d->q && aligned16(d->q) && strides_ok(d->sq, d->B, d->Nq, d->H), "%s: q: 16-byte alignment of the pointer and of every stride, token stride below 2^24", who);
   if (d->Nk > 0 && d->B > 0)
@@ -1354,11 +1357,11 @@ __global__ void xattn_zero_kernel(uint16_t* dst, Strides s, int64_t n, int N, in
 }  // namespace
 
 extern "C" int64_t lt_cross_attention_fwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh) {
-  if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 128) return 0;
+  if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 128 || !in_range(B, Nq, Nk, H, Hkv)) return 0;
   return fwd_floats(B, Nq * (H / Hkv), Nk, Hkv, dh);
 }
 extern "C" int64_t lt_cross_attention_bwd_ws_floats(int B, int Nq, int Nk, int H, int Hkv, int dh) {
-  if (B <= 0 || Nq <= 0 || Nk < 0 || H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 128) return 0;
+  if (B <= 0 || Nq <= 0 || Nk < 0 || H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 128 || !in_range(B, Nq, Nk, H, Hkv)) return 0;
   return bwd_floats(B, Nq * (H / Hkv), Nk, Hkv, dh);
 }
 
