@@ -1202,17 +1202,21 @@ int split_for(int64_t blocks, int chunks, int per_cu, double us_step, double mby
   return best;
 }
 bool few_rows(int R) { return R <= 32; }
-// Workgroups that a CU holds (registers) and the measured us of a 64-token chunk with that many on it, per 32 columns of head_dim:
+// Workgroups that a CU holds (registers; head_dim <= 32 one more than is counted here) and the measured us of a 64-token chunk with that many on it, per
+// 32 columns of head_dim:
 //   forward, one 32-row tile a wave     3 at head_dim <= 64: 1.15, 2 above: 0.63
 //   forward, two tiles a wave           2 at head_dim <= 64: 1.38 (they share every K / V fragment read from LDS: 15 % more rows per us when the card is full)
-//   dQ                                  3 at head_dim <= 64: 1.4,  2 above: 1.6;   dK / dV   2 at head_dim <= 64: 1.15, 1 above: 1.6
-// The few-row kernels walk 128 keys a step: 1.5 us (forward, 3 workgroups a CU), 2.5 us (backward, 2).
+//   dQ                                  3 at head_dim <= 64: 1.4,  2 up to 96: 1.6, 1 above: 1.0;   dK / dV   2 at head_dim <= 64: 1.15, 1 above: 1.6
+// The few-row kernels walk 128 keys a step: 1.5 us (forward; 3 workgroups a CU, 2 above head_dim 64), 2.5 us (backward, 2), 5 us (backward above 64, 1).
+// Priced with one more workgroup a CU than is there, head_dim 128 took (both swept): dQ of 8 x 196 x 1370 x 12 heads 169 us in two cuts against 154 uncut; the
+// one-query forward of 16 x 1370 x 12 heads 33 us in four against 27 uncut; 16 x 100 x 1025 x 8 heads with resident rows 103 in three against 91 in two.  (The
+// one that lost by the right count: the one-query forward of 32 x 1370 x 12 heads, 57 -> 64.)
 Plan fwd_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int64_t bh = (int64_t)B * Hkv;
   const int HD = lt_cdiv(dh, 32), chunks = lt_cdiv(Nk, KC);
   const double mb = 4e-6 * bh * R * dh;
   double t1, t2;
-  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 3, 1.5, mb, t1)};
+  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), HD <= 2 ? 3 : 2, 1.5, mb, t1)};
   const int n1 = lt_cdiv(R, 128), n2 = lt_cdiv(R, 256);
   const int s1 = split_for(bh * n1, chunks, HD <= 2 ? 3 : 2, (HD <= 2 ? 1.15 : 0.63) * HD, mb, t1);
   if (HD > 2) return {false, n1, 1, s1};
@@ -1224,8 +1228,8 @@ Plan dq_plan(int B, int R, int Nk, int Hkv, int dh) {
   const int HD = lt_cdiv(dh, 32), tiles = lt_cdiv(R, 128);
   const double mb = 4e-6 * bh * R * dh;
   double t;
-  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), 2, 2.5, mb, t)};
-  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(Nk, KC), HD <= 2 ? 3 : 2, (HD <= 2 ? 1.4 : 1.6) * HD, mb, t)};
+  if (few_rows(R)) return {true, 1, 1, split_for(bh, lt_cdiv(Nk, 128), HD <= 2 ? 2 : 1, HD <= 2 ? 2.5 : 5., mb, t)};
+  return {false, tiles, 1, split_for(bh * tiles, lt_cdiv(Nk, KC), HD <= 2 ? 3 : HD == 3 ? 2 : 1, HD <= 2 ? 1.4 * HD : HD == 3 ? 4.8 : 4., mb, t)};
 }
 int resident_rows(int HD) { return HD == 1 ? rows_resident<1>() : HD == 2 ? rows_resident<2>() : HD == 3 ? rows_resident<3>() : rows_resident<4>(); }
 Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
@@ -1234,9 +1238,10 @@ Plan dkdv_plan(int B, int R, int Nk, int Hkv, int dh) {
   double t;
   if (R <= resident_rows(HD)) {   // no partials to join: cut the keys until the rounds are even; ~4 us to stage the rows, 4 tiles a step
     Plan p{true, 1, 1, 1};
+    const int held = (HD <= 2 ? 2 : 1) * CUS;
     double least = 1e30;
-    for (int s = 1; s <= tiles && (s == 1 || bh * s <= 16 * 2 * CUS); ++s) {   // (16 rounds: more cuts only stage the rows again)
-      const double u = (double)((bh * s + 2 * CUS - 1) / (2 * CUS)) * (4. + 0.4 * HD * lt_cdiv(R, 32) * (double)((tiles + s - 1) / s));
+    for (int s = 1; s <= tiles && (s == 1 || bh * s <= 16 * held); ++s) {   // (16 rounds: more cuts only stage the rows again)
+      const double u = (double)((bh * s + held - 1) / held) * (4. + 0.4 * HD * lt_cdiv(R, 32) * (double)((tiles + s - 1) / s));
       if (u < least) { least = u; p.splits = s; }
     }
     return p;
