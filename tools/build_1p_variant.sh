@@ -9,7 +9,7 @@ W=${TMPDIR:-/tmp}/lt_1p_variant
 mkdir -p $W/obj
 for f in gemm.hip gemm_p.hip gemm_args.h; do git -C $R show db361e8^:lightly-train_amd/csrc/$f > $W/$f; done
 python $R/__graft_entry__.py > /dev/null
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wno-unused-result -I$W -I$R/lightly-train_amd/csrc -I$R/include -x hip"
+F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -I$W -I$R/lightly-train_amd/csrc -I$R/include -x hip"
 hipcc $F -c $W/gemm.hip -o $W/obj/gemm_old.o
 hipcc $F -c $W/gemm_p.hip -o $W/obj/gemm_p.o
 OBJS=$(ls $R/lightly-train_amd/lib/obj/*.o | grep -v "gemm.hip.o\|gemm_timing.o\|gemm_f32nt.o")

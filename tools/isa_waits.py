@@ -20,7 +20,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 def compile_to_isa(src: str) -> str:
     out = os.path.join(tempfile.mkdtemp(prefix="lt_isa_"), "k.s")
-    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-I", os.path.join(ROOT, "include"),
+    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+           "-I", os.path.join(ROOT, "include"),
            "-I", os.path.join(ROOT, "lightly-train_amd", "csrc"), "-S", "--cuda-device-only", "-o", out, src]
     subprocess.run(cmd, check=True, stderr=subprocess.DEVNULL)
     return out

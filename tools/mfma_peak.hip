@@ -1,6 +1,6 @@
 // Practical MFMA ceiling of the chip (measurement tool): v_mfma_f32_32x32x16_bf16 issued back to back from registers, no
 // memory traffic, on every SIMD of every CU -- what "100 % MFMA" means on this part at the clock it sustains under that load.
-//   hipcc --offload-arch=gfx950 -O3 -o tools/mfma_peak tools/mfma_peak.hip && tools/mfma_peak
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/mfma_peak tools/mfma_peak.hip && tools/mfma_peak
 // Variants: waves per SIMD (1, 2), independent accumulator chains per wave (1, 2, 4); also a dependent v_fma chain to read
 // the shader clock (one wave64 VALU op issues in 4 cycles... measured as ops/s) with the chip idle and under MFMA load.
 #include <hip/hip_runtime.h>
