@@ -16,7 +16,8 @@
 //
 // Roundings to 16 bits: the tiled kernels round P and dS once on their way into the second product, which makes a result's error sqrt(2) of its own rounding
 // (measured 1.1 - 1.4 for O, 1.4 for dV, 1.4 - 1.5 for dK and 1.4 - 1.57 for dQ, to which D from the rounded O adds); both halves of dS would cost dQ
-// a third more matrix work.  The few-row kernels, which memory bounds, multiply both halves (measured 1.00, dQ <= 1.06).
+// a third more matrix work.  The few-row kernels, which memory bounds, multiply both halves (measured 1.00, dQ <= 1.08).  f16 factors are brought into
+// the type's range first (P_LOG2, P_UP, DS_UP): the same figures hold there, at every upstream scale.
 #include "lt_common.h"
 
 namespace {

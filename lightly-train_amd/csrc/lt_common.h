@@ -111,7 +111,7 @@ __device__ __forceinline__ float gelu_grad_f(float x) {
 
 // The same evaluation on a PAIR of values; constants folded (1/sqrt2 into p, 1/2 into the polynomial, -log2(e)/2 into the exponent:
 // v_exp_f32 is a base-2 exponential).  The GELU epilogues of the token GEMMs are VALU-bound, not HBM-bound -- storing the pre-activations as
-// a second output costs nothing, the GELU arithmetic cost 72 us of a 391-us fc1 launch (tools/gelu_probe.py) -- so issue slots are what the
+// a second output costs nothing, the GELU arithmetic costs 94 us of a 340-us fc1 launch (tools/gelu_probe.py) -- so issue slots are what the
 // folding buys.  (The library is built without packed fp32 instructions: a pair is two scalar chains.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_parts2(f32x2 x, f32x2& h, f32x2& ex) {   // h = erfc(|x| / sqrt2) / 2,  ex = exp(-x^2 / 2)

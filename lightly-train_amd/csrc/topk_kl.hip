@@ -6,9 +6,11 @@
 //   dlogits = w / T * { m q_j - p_j  kept;  q_i (m - p_rest / q_rest)  others },   m = sum p_j + p_rest
 // m is 1 wherever there is a bucket (p_rest = 1 - sum p_j) and for renormalised values.  Kept probabilities whose sum passes 1 (values stored in 16 bits next to a
 // 32-bit t_lse: up to 1.04 for a sure teacher), or rows of which every class is kept, have no bucket: there m = sum p_j, or the gradient were not the loss's.
-// Bound by memory: the row is read once and its gradient written once.  The registers of a workgroup of 512 threads hold a row of up to 65 536 fp32 (32
-// pieces of 16 bytes a thread) between the three passes over it (maximum, sum of exponentials, gradient); what does not fit is read again, through the
-// caches (a sixteenth of the row costs ~10 us at 2048 x 65 536).  One workgroup to a CU walks the rows and requests each piece of the next row behind
+// Bound by memory: the row is read once and its gradient written once.  The registers of a workgroup of 512 threads hold a row of up to 65 536 fp32 or 16-bit
+// values (32 or 16 pieces of 16 bytes a thread) between the three passes over it (maximum, sum of exponentials, gradient); what does not fit is read again,
+// through the caches (a sixteenth of the row costs ~10 us at 2048 x 65 536).  Spilled beside them: 10 registers a lane of row-long values and descriptors in the
+// fp32 form, 13 - 17 in the 16-bit forms (12 for their short rows), 2 - 8 where rows are not whole pieces; what that costs was not separated.  Rates reached
+// elsewhere: 16-bit rows of 65 536 2.9 TB/s, of 131 072 (half of it streamed) 2.6; 1024 x 50 257 (one element a load) fp32 2.3, bf16 1.7.  One workgroup to a CU walks the rows and requests each piece of the next row behind
 // the store of this one's: 2048 x 65 536 fp32 -> bf16 with 256 kept, 207 us (3.9 TB/s of the 5.0 that a copy reaches; one row a workgroup: 246 us).
 // The classes not kept are summed on their own (a bitmap in LDS says which are) against their own maximum: q_rest as 1 - sum of the kept q would
 // cancel, and p_rest is formed in 64 bits for the same reason.  The kept classes' gradients overwrite the row's after a barrier.
