@@ -126,3 +126,34 @@ def test_products_past_the_largest_f16_number_are_no_infinities(Nq, Nk, dh):
     dP = torch.matmul(v[0, :, 0].double(), do[0, -1, 0].double())
     assert (P * (dP - (P * dP).sum())).abs().max() > 65504 and all(x.abs().max() < 60000 for x in want)
     _assert_roundings(_backward(q, k, v, do, scale), want)
+
+
+@pytest.mark.parametrize("Nq,Nk", [(2, 900), (100, 900), (300, 2000)])
+def test_replayed_graphs_find_their_scales_anew(Nq, Nk):
+    """One captured pass, replayed over upstream gradients of other sizes with eager calls between: nothing of one replay's powers of two reaches the next."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    q, k, v, do = rnd(2, Nq, 2, 64).to(HF), rnd(2, Nk, 2, 64).to(HF), rnd(2, Nk, 2, 64).to(HF), rnd(2, Nq, 2, 64).to(HF)
+    o = [torch.empty_like(q), torch.empty(2, 2, Nq, device="cuda"), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]
+    ws = torch.empty(max(ops.cross_attention_fwd_ws_floats(2, Nq, Nk, 2, 2, 64), ops.cross_attention_bwd_ws_floats(2, Nq, Nk, 2, 2, 64)), device="cuda")
+
+    def run():
+        ops.cross_attention_fwd(q, k, v, o[0], o[1], 0.125, ws=ws)
+        ops.cross_attention_bwd(q, k, v, o[0], do, o[1], o[2], o[3], o[4], 0.125, ws=ws)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    base = do.float()
+    for size in (1e3, 1e-3, 1.0, 1e3, 1e-4):
+        do.copy_((base * size).to(HF))
+        want = _backward(q, k, v, do, 0.125)
+        for t in (*o, ws):
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((o[0], *o[2:]), want):
+            assert torch.equal(a, b), size
