@@ -313,6 +313,7 @@ int lt_kl_fwd_bwd(const float* s_logits, const float* t_logits, int ld, float in
  *   loss_rows[r] = w * (sum_j p_j log(p_j / q_j) + p_rest log(p_rest / q_rest));  loss[0] += sum_r loss_rows[r] (loss may be NULL; order-fixed)
  *   dlogits[r]   = w * inv_temp * (m q_j - p_j on kept classes, q_i * (m - p_rest / q_rest) elsewhere), m = sum_j p_j + p_rest       (dlogits may be NULL)
  * (m is 1 except where the kept probabilities pass 1, as values stored in 16 bits may beside a 32-bit t_lse, or where every class is kept: m = sum_j p_j)
+ * (inv_temp and t_lse are 32-bit numbers: p_rest is known to about 2^-24 (|t_lse| + |t_val * inv_temp|))
  * An index outside 0 .. K - 1 is a missing entry; of an index that comes again in its row the first entry counts; a row without entries, of weight 0
  * or (without t_lse) with all entries -inf gives loss 0 and gradient 0.  A NaN among a row's entries or logits shows in its loss and gradient.
  *   s rows ld apart, LT_DT_*; dlogits rows ldd apart, the type of s, or bf16 for f32 s; t_val LT_DT_* rows ldv apart; t_idx int32 or (idx_is_64)
